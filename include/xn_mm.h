@@ -371,6 +371,65 @@ int xn_mm_kv_append2(xn_dtype dtype, void *k_cache, void *v_cache, const void *k
                      size_t src_batch_stride, const int64_t *index, size_t batch, size_t heads, size_t context,
                      size_t head_dim, void *stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A serving step around the linears (no counterpart among the reference's kernels beyond its rope): rotary positions, a
+ * cache of pages shared by all sequences, attention over it, and the draw of the next token.
+ *
+ * The cache is two pools (num_pages, kv_heads, page_size, head_dim) with common strides (elements; the last dimension
+ * contiguous).  Token j of a sequence lies in row j % page_size of page page_table[sequence][j / page_size]; its slot is
+ * page * page_size + row.
+ * ------------------------------------------------------------------------------------------ */
+/* Rotary positions: dst[t][h] = src[t][h] with pair j of the first `rotated` elements turned by positions[t] * freqs[j] radians
+ * (rotated / 2 frequencies, 64-bit: the angle is formed in 64 bits, so far positions lose nothing).  interleaved: pairs are
+ * elements (2 j, 2 j + 1) (rope_i, xn-core/src/backend.rs), otherwise (j, j + rotated / 2) (rope).  The rest of each head of head_dim
+ * elements is copied.  f32 math, one rounding.  Any strides with contiguous heads; dst may be src with the same strides,
+ * and must not overlap it otherwise. */
+int xn_mm_rope(xn_dtype dtype, void *dst, size_t dst_token_stride, size_t dst_head_stride, const void *src, size_t src_token_stride,
+               size_t src_head_stride, const int64_t *positions, const double *freqs, size_t tokens, size_t heads, size_t head_dim,
+               size_t rotated, int interleaved, void *stream);
+/* The new tokens of a batch go into the cache: k is turned like xn_mm_rope and written to its slot, v is written as it is, and
+ * q (when q_dst is not null: contiguous (tokens, heads, head_dim)) is turned on the way -- one launch over the rows of the fused
+ * projection.  freqs null: nothing is turned.  A slot outside [0, num_pages * page_size) stores nothing (padding);
+ * the slots of one call are distinct.  What else the pools hold stays as it is. */
+int xn_mm_paged_append(xn_dtype dtype, void *k_pages, void *v_pages, size_t page_stride, size_t head_stride, size_t row_stride,
+                       size_t num_pages, size_t page_size, const void *k, size_t k_token_stride, size_t k_head_stride, const void *v,
+                       size_t v_token_stride, size_t v_head_stride, const int64_t *slots, size_t tokens, size_t kv_heads,
+                       size_t head_dim, void *q_dst_or_null, const void *q, size_t q_token_stride, size_t q_head_stride, size_t heads,
+                       const int64_t *positions, const double *freqs_or_null, size_t rotated, int interleaved, void *stream);
+/* Attention of the newest tokens of `batch` sequences over the paged cache that already holds their keys and values.
+ * Sequence b has the query rows [query_starts[b], query_starts[b + 1]) of q (query_starts null: row b alone) and context[b] keys
+ * with them; its row i of n sees key j iff j <= i + context[b] - n and, where window > 0, j > i + context[b] - n - window:
+ *   out[t][h] = softmax_j(scale * q[t][h] . k[j][h / (heads / kv_heads)]) v[j][...]
+ * A row that sees nothing is zeros; rows of q that belong to no sequence leave out as it is.  16-bit elements, head_dim 64 or
+ * 128, any page size, 16-byte aligned tensors with strides in multiples of 8 elements.  Scores, softmax statistics and the output's sum
+ * are f32; the probabilities are rounded to the element type for the second product.  max_query: an upper bound of the rows of a
+ * sequence, by which the kernel is chosen (0: unknown); results hold for any.
+ * Lengths and indexes are device memory that the host does not see: a length is bounded by the tensors, and a page index outside
+ * [0, num_pages) reads as a page of zeros.  What pages hold beyond a sequence's context is never used.  A key or value
+ * inside the context that is not finite may reach those rows, of the same call and key head, that do not see it.
+ * workspace: xn_mm_attention_paged_workspace_bytes(head_dim) bytes of device memory, 256-byte aligned, owned by the
+ * caller; calls that may overlap need one each. */
+size_t xn_mm_attention_paged_workspace_bytes(size_t head_dim);
+int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token_stride, size_t out_head_stride, const void *q,
+                          size_t q_token_stride, size_t q_head_stride, size_t tokens, size_t heads, const void *k_pages,
+                          const void *v_pages, size_t page_stride, size_t head_stride, size_t row_stride, size_t num_pages,
+                          size_t page_size, size_t kv_heads, size_t head_dim, const int32_t *page_table, size_t table_stride,
+                          size_t max_pages, const int32_t *context, const int32_t *query_starts_or_null, size_t batch,
+                          size_t max_query, size_t window, float scale, void *workspace, size_t workspace_bytes, void *stream);
+/* The next token of every row of logits (rows row_stride elements apart, up to 2^20 logits each).  With the tokens in
+ * falling order of their logit (equal ones in rising order of index) and w = exp((logit - largest) / temperature):
+ *   top_k  (> 0)  keeps the first top_k;
+ *   top_p  (< 1)  of those, keeps each while the weights before it sum to less than top_p times the sum of them all, the first always;
+ *   min_p  (> 0)  keeps those with w >= min_p, the first always;
+ * tokens[r] is the first kept token, in order of index, at which the running sum of kept weights exceeds uniform[r] (in [0, 1))
+ * times their total.  A temperature that is not positive takes the largest logit, of equal ones the lowest index.  Logits of
+ * -inf and NaN are never drawn; a row of nothing else gives -1.  Weights are summed exactly, as multiples of 2^-42: the result depends
+ * on nothing but the inputs.  The settings are one value per row, f32 (top_k int32); a null pointer leaves the filter off
+ * (temperature: 1). */
+int xn_mm_sample(xn_dtype dtype, int64_t *tokens, const void *logits, size_t row_stride, size_t rows, size_t vocab, const float *uniform,
+                 const float *temperature_or_null, const int32_t *top_k_or_null, const float *top_p_or_null,
+                 const float *min_p_or_null, void *stream);
+
 /* Allocation-free form of xn_mm_linear_fp8.  It has no counterpart in the reference.  For hosts
  * that must not (or cannot) allocate device memory at call time -- a serving loop whose device
  * budget belongs to another allocator, a real-time audio callback that cannot afford a

@@ -141,6 +141,30 @@ extern "C" {
     pub fn xn_mm_kv_append2(dtype: XnDtype, k_cache: *mut c_void, v_cache: *mut c_void, k_src: *const c_void,
         v_src: *const c_void, src_batch_stride: usize, index: *const i64, batch: usize, heads: usize,
         context: usize, head_dim: usize, stream: *mut c_void) -> c_int;
+    pub fn xn_mm_rope(dtype: XnDtype, dst: *mut c_void, dst_token_stride: usize, dst_head_stride: usize,
+        src: *const c_void, src_token_stride: usize, src_head_stride: usize, positions: *const i64,
+        freqs: *const f64, tokens: usize, heads: usize, head_dim: usize, rotated: usize,
+        interleaved: c_int, stream: *mut c_void) -> c_int;
+    pub fn xn_mm_paged_append(dtype: XnDtype, k_pages: *mut c_void, v_pages: *mut c_void, page_stride: usize,
+        head_stride: usize, row_stride: usize, num_pages: usize, page_size: usize, k: *const c_void,
+        k_token_stride: usize, k_head_stride: usize, v: *const c_void, v_token_stride: usize,
+        v_head_stride: usize, slots: *const i64, tokens: usize, kv_heads: usize, head_dim: usize,
+        q_dst_or_null: *mut c_void, q: *const c_void, q_token_stride: usize, q_head_stride: usize,
+        heads: usize, positions: *const i64, freqs_or_null: *const f64, rotated: usize,
+        interleaved: c_int, stream: *mut c_void) -> c_int;
+    pub fn xn_mm_attention_paged_workspace_bytes(head_dim: usize) -> usize;
+    pub fn xn_mm_attention_paged(dtype: XnDtype, out: *mut c_void, out_token_stride: usize,
+        out_head_stride: usize, q: *const c_void, q_token_stride: usize, q_head_stride: usize,
+        tokens: usize, heads: usize, k_pages: *const c_void, v_pages: *const c_void, page_stride: usize,
+        head_stride: usize, row_stride: usize, num_pages: usize, page_size: usize, kv_heads: usize,
+        head_dim: usize, page_table: *const i32, table_stride: usize, max_pages: usize,
+        context: *const i32, query_starts_or_null: *const i32, batch: usize, max_query: usize,
+        window: usize, scale: f32, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn xn_mm_sample(dtype: XnDtype, tokens: *mut i64, logits: *const c_void, row_stride: usize,
+        rows: usize, vocab: usize, uniform: *const f32, temperature_or_null: *const f32,
+        top_k_or_null: *const i32, top_p_or_null: *const f32, min_p_or_null: *const f32,
+        stream: *mut c_void) -> c_int;
     pub fn xn_mm_linear_fp8_noalloc_max_elems() -> usize;
     pub fn xn_mm_linear_fp8_noalloc(y_bf16: *mut c_void, x_bf16: *const c_void, wq: *const u8,
         w_scale: *const f32, m: usize, n: usize, k: usize, variant: c_int, stream: *mut c_void) -> c_int;

@@ -15,6 +15,6 @@ from . import _host  # noqa: E402  built beside the library; like it, without a 
 _host.set_error_class(XnError)
 
 from . import ops  # noqa: E402
-from .ops import (Linear, LinearFp8, LinearQ4, gemm, linear_fp8, linear_q4, matmul, matmul_, matmul_plan,  # noqa: E402
+from .ops import (Linear, LinearFp8, LinearQ4, attention_paged, gemm, linear_fp8, linear_q4, matmul, matmul_, matmul_plan,  # noqa: E402
                   matmul_t, matmul_with_t, quantize_rows_i8, quantize_weights_fp8, quantize_weights_q4, quantize_weights_q8, linear_q8,
-                  split_rows_e4m3)
+                  paged_append_, rope, rope_frequencies, sample, split_rows_e4m3)

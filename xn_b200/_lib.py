@@ -78,6 +78,11 @@ SIGNATURES = {
     "xn_mm_gemm_causal": (_i, [_i, _sz, _i, _p, _p, _sz, _p, _sz] + [_sz] * 12 + [_p]),
     "xn_mm_attention_prefill": (_i, [_i, _p, _sz, _p, _p, _p, _sz, _sz, _sz, _sz, _sz, _sz, C.c_float, _p]),
     "xn_mm_scatter_columns": (_i, [_p, _sz, _i, _sz, _sz, _p, _sz, _sz, _sz, _p]),
+    "xn_mm_rope": (_i, [_i, _p, _sz, _sz, _p, _sz, _sz, _p, _p, _sz, _sz, _sz, _sz, _i, _p]),
+    "xn_mm_paged_append": (_i, [_i, _p, _p] + [_sz] * 5 + [_p, _sz, _sz, _p, _sz, _sz, _p, _sz, _sz, _sz, _p, _p, _sz, _sz, _sz, _p, _p, _sz, _i, _p]),
+    "xn_mm_attention_paged_workspace_bytes": (_sz, [_sz]),
+    "xn_mm_attention_paged": (_i, [_i, _p, _sz, _sz, _p, _sz, _sz, _sz, _sz, _p, _p] + [_sz] * 7 + [_p, _sz, _sz, _p, _p, _sz, _sz, _sz, C.c_float, _p, _sz, _p]),
+    "xn_mm_sample": (_i, [_i, _p, _p, _sz, _sz, _sz, _p, _p, _p, _p, _p, _p]),
     "xn_mm_linear_fp8_noalloc_max_elems": (_sz, []),
     "xn_mm_linear_fp8_noalloc": (_i, [_p, _p, _p, _p, _sz, _sz, _sz, _i, _p]),
 }

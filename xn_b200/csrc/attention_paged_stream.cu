@@ -1,0 +1,536 @@
+// Attention of few query rows over a paged cache: the keys and values stream through once, from HBM.
+//
+// Work is counted in units of 16 keys of one (sequence, tile of rows, key head) item, all items laid end to end, and dealt out
+// evenly to the warps of the machine, whatever the lengths: a long context is shared by many warps, short ones follow one
+// another in a warp.  The rows of an item are the query heads of one key head, for one or more tokens: up to 8 x NT of them.
+//
+// A warp keeps its own ring of units in shared memory, filled with 16-byte asynchronous copies (rows of a unit may lie in any
+// pages) and never waits for another warp while it streams.  Per unit, on mma.sync:
+//   S^T = K Q^T   16 keys x 8 rows per product, Q's fragments stay in registers
+//   running maximum and sum of every row (a lane owns two rows' columns), p = 2^(s - m)
+//   O^T += V^T P^T, V's fragments by transposing loads, P^T turned in registers
+// Keys ride the 16-row dimension, rows the 8-column one: with one to eight rows (a token's heads) half of what the other way
+// round would cost, which keeps the products well below the time that the unit's bytes take to arrive.  P is rounded to the
+// element type for the second product (relative 2^-9 of each, as the output's own rounding); scores, maxima, sums and O stay
+// in f32.
+//
+// A warp that holds the whole of an item writes its rows; parts are joined within the CTA through shared memory, and what
+// crosses CTAs (at most two records of each) by a second kernel.
+#include "paged.cuh"
+
+namespace xn {
+namespace {
+
+__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(unsigned dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ unsigned transpose8x8(unsigned x) {
+    unsigned y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
+template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+constexpr int UNIT = 16;  // keys
+
+// The units of a sequence: kv_heads * tiles items of U units each.
+struct SequenceUnits {
+    Sequence s;
+    int lo;      // first key that any row sees
+    int base;    // the same, down to a multiple of the unit
+    int U, tiles;
+    __device__ __forceinline__ unsigned long long total(const PagedArgs &a) const {
+        return (unsigned long long)U * (unsigned)tiles * (unsigned)a.kv_heads;
+    }
+};
+template <int TR> __device__ __forceinline__ SequenceUnits sequence_units(const PagedArgs &a, int b) {
+    SequenceUnits u;
+    u.s = load_sequence(a, b);
+    u.lo = a.window ? max(0, u.s.off + 1 - a.window) : 0;
+    u.base = u.lo / UNIT * UNIT;
+    u.U = max(1, (u.s.ctx - u.base + UNIT - 1) / UNIT);  // rows that see nothing get their zeros from an empty unit
+    u.tiles = (int)(((long long)u.s.n * a.group + TR - 1) / TR);
+    return u;
+}
+
+// A place in the line of all units.
+struct Cursor {
+    unsigned long long pos;
+    int b, head, tile, unit;
+    SequenceUnits u;
+};
+template <int TR> __device__ __forceinline__ void next_sequence(const PagedArgs &a, Cursor &c) {
+    for (++c.b; c.b < a.batch; ++c.b) {
+        c.u = sequence_units<TR>(a, c.b);
+        if (c.u.tiles) break;
+    }
+    c.head = c.tile = c.unit = 0;
+}
+template <int TR> __device__ __forceinline__ void advance(const PagedArgs &a, Cursor &c) {
+    ++c.pos;
+    if (++c.unit < c.u.U) return;
+    c.unit = 0;
+    if (++c.tile < c.u.tiles) return;
+    c.tile = 0;
+    if (++c.head < a.kv_heads) return;
+    next_sequence<TR>(a, c);
+}
+
+// One warp's or CTA's part of an item, in shared memory: O [rows][HD], then m, l
+struct PartHead {
+    unsigned long long begin, end;  // units of the item; end == 0: none
+    int q0, rows, tile_row, head;
+};
+
+template <typename T, int HD, int NT, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const PagedArgs a) {
+    constexpr int TR = 8 * NT, CHUNKS = HD / 8, ROWS_AT_ONCE = 32 / CHUNKS;
+    constexpr int ROW_BYTES = HD * 2, TILE = UNIT * ROW_BYTES, STAGE = 2 * TILE;
+    constexpr int REC = TR * (HD + 2);
+    static_assert(REC * 4 <= STAGES * STAGE, "a warp's last part takes the place of its ring");
+    extern __shared__ __align__(1024) unsigned char smem[];
+    float *recs = reinterpret_cast<float *>(smem + WARPS * STAGES * STAGE);  // first parts, one per warp
+    __shared__ unsigned long long scan[WARPS + 1];
+    __shared__ unsigned long long start_base[WARPS];
+    __shared__ int start_b[WARPS];
+    __shared__ PartHead heads[2 * WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    dependent_begin();
+
+    // ---- where every warp's share begins: all sequences' units, added up in order ----
+    unsigned long long total = 0;
+    auto block_scan = [&](unsigned long long x, unsigned long long &sum) {  // exclusive
+        unsigned long long inc = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = inc;
+        __syncthreads();
+        unsigned long long before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += scan[w];
+            all += scan[w];
+        }
+        sum = all;
+        return before + inc - x;
+    };
+    const int rounds = (a.batch + WARPS * 32 - 1) / (WARPS * 32);
+    unsigned long long mine = 0, at = 0;
+    for (int r = 0; r < rounds; ++r) {
+        const int b = r * WARPS * 32 + (int)threadIdx.x;
+        mine = b < a.batch ? sequence_units<TR>(a, b).total(a) : 0;
+        unsigned long long sum;
+        at = block_scan(mine, sum);
+        total += sum;
+    }
+    const unsigned shares = gridDim.x * WARPS, share = blockIdx.x * WARPS + warp;
+    unsigned long long seen = 0;
+    for (int r = 0; r < rounds; ++r) {
+        const int b = r * WARPS * 32 + (int)threadIdx.x;
+        unsigned long long sum = total;
+        if (rounds > 1) {
+            mine = b < a.batch ? sequence_units<TR>(a, b).total(a) : 0;
+            at = block_scan(mine, sum);
+        }
+        for (int w = 0; w < WARPS; ++w) {
+            const unsigned long long p = share_begin(total, blockIdx.x * WARPS + w, shares);
+            if (p >= seen + at && p < seen + at + mine) {
+                start_b[w] = b;
+                start_base[w] = seen + at;
+            }
+        }
+        seen += sum;
+    }
+    if (lane == 0) heads[2 * warp].end = heads[2 * warp + 1].end = 0;
+    __syncthreads();
+    const unsigned long long first = share_begin(total, share, shares), last = share_begin(total, share + 1, shares);
+
+    unsigned char *ring = smem + warp * STAGES * STAGE;
+    auto store_part = [&](int which, const Cursor &c, const float (&o)[HD / 16][NT][4], const float (&m)[NT][2], const float (&l)[NT][2]) {
+        float *rec = which == 0 ? recs + warp * REC : reinterpret_cast<float *>(ring);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = nt * 8 + (lane & 3) * 2 + e;
+#pragma unroll
+                for (int mt = 0; mt < HD / 16; ++mt) {
+                    rec[row * HD + mt * 16 + (lane >> 2)] = o[mt][nt][e];
+                    rec[row * HD + mt * 16 + 8 + (lane >> 2)] = o[mt][nt][2 + e];
+                }
+                if (lane < 4) {
+                    rec[TR * HD + row] = m[nt][e];
+                    rec[TR * HD + TR + row] = l[nt][e];
+                }
+            }
+    };
+    if (first < last) {
+        Cursor pc;  // what is loaded next
+        pc.pos = first;
+        pc.b = start_b[warp];
+        pc.u = sequence_units<TR>(a, pc.b);
+        {
+            const unsigned long long rem = first - start_base[warp];
+            const unsigned item = (unsigned)(rem / (unsigned)pc.u.U);
+            pc.unit = (int)(rem % (unsigned)pc.u.U);
+            pc.head = (int)(item / (unsigned)pc.u.tiles);
+            pc.tile = (int)(item % (unsigned)pc.u.tiles);
+        }
+        Cursor cc = pc;  // what is computed next
+        int page = -1;   // the page of this lane's key in the unit at pc: read one unit ahead
+        auto key_of = [&](const Cursor &c) { return c.u.base + c.unit * UNIT + (lane & 15); };
+        auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : (int)((unsigned)key / (unsigned)a.page_size); };
+        auto fetch_page = [&]() {
+            page = -1;
+            if (pc.pos < last) {
+                const int key = key_of(pc);
+                if (key >= pc.u.lo && key < pc.u.s.ctx) page = a.table[(long long)pc.b * a.table_stride + page_of(key)];
+            }
+        };
+        auto issue = [&](int slot) {
+            if (pc.pos < last) {
+                const int key = key_of(pc);
+                const bool there = page >= 0 && page < a.num_pages;
+                const long long at_row = there ? (long long)page * a.page_stride + (long long)pc.head * a.head_stride +
+                                                     (long long)(key - page_of(key) * a.page_size) * a.row_stride
+                                               : -1;
+                const unsigned kdst = smem_addr(ring + slot * STAGE), vdst = kdst + TILE;
+                const int chunk = lane % CHUNKS;
+#pragma unroll
+                for (int i = 0; i < UNIT / ROWS_AT_ONCE; ++i) {
+                    const int row = i * ROWS_AT_ONCE + lane / CHUNKS;
+                    const long long off = __shfl_sync(0xffffffffu, at_row, row);
+                    const bool valid = off >= 0;
+                    const long long e = valid ? off + chunk * 8 : 0;
+                    const unsigned d = (unsigned)(row * ROW_BYTES + ((chunk ^ (row & 7)) << 4));
+                    cp_async16(kdst + d, static_cast<const T *>(a.k) + e, valid);
+                    cp_async16(vdst + d, static_cast<const T *>(a.v) + e, valid);
+                }
+                advance<TR>(a, pc);
+                fetch_page();
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch_page();
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) issue(s);
+
+        unsigned qf[HD / 16][NT][2];
+        float o[HD / 16][NT][4], m[NT][2], l[NT][2];
+        int hi_key[NT][2], lo_key[NT][2];
+        bool fresh = true;
+        unsigned long long item_begin = 0;
+        int slot = 0;
+        while (cc.pos < last) {
+            if (fresh) {
+                fresh = false;
+                item_begin = cc.pos - (unsigned)cc.unit;
+                const int rows = (int)min((long long)cc.u.s.n * a.group - (long long)cc.tile * TR, (long long)TR);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int rq = nt * 8 + (lane >> 2);  // the row of this lane's Q fragments
+                    const unsigned r = (unsigned)(cc.tile * TR + rq);
+                    const T *qp = static_cast<const T *>(a.q) + (long long)(cc.u.s.q0 + (int)(r / (unsigned)a.group)) * a.q_token +
+                                  (long long)(cc.head * a.group + (int)(r % (unsigned)a.group)) * a.q_head + (lane & 3) * 2;
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        qf[kk][nt][0] = rq < rows ? *reinterpret_cast<const unsigned *>(qp + kk * 16) : 0u;
+                        qf[kk][nt][1] = rq < rows ? *reinterpret_cast<const unsigned *>(qp + kk * 16 + 8) : 0u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int rs = nt * 8 + (lane & 3) * 2 + e;  // the row of this lane's scores
+                        const int i = (int)((unsigned)(cc.tile * TR + rs) / (unsigned)a.group);
+                        hi_key[nt][e] = rs < rows ? min(cc.u.s.ctx - 1, cc.u.s.off + i) : -1;
+                        lo_key[nt][e] = a.window ? cc.u.s.off + i - a.window + 1 : 0;
+                        m[nt][e] = -INFINITY;
+                        l[nt][e] = 0.0f;
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < HD / 16; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[mt][nt][e] = 0.0f;
+                }
+            }
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();
+            issue(slot == 0 ? STAGES - 1 : slot - 1);  // the slot of the unit before this one
+
+            const unsigned kt = smem_addr(ring + slot * STAGE), vt = kt + TILE;
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                unsigned kf[4];
+                const int row = lane & 15, chunk = kk * 2 + (lane >> 4);
+                ldmatrix_x4(kf, kt + row * ROW_BYTES + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<T>(s[nt], kf, qf[kk][nt][0], qf[kk][nt][1]);
+            }
+            const int key0 = cc.u.base + cc.unit * UNIT + (lane >> 2), key1 = key0 + 8;
+            unsigned pf[NT][2];
+            bool moved = false;
+            float alpha[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x0 = key0 <= hi_key[nt][e] && key0 >= lo_key[nt][e] ? s[nt][e] * a.c : -INFINITY;
+                    const float x1 = key1 <= hi_key[nt][e] && key1 >= lo_key[nt][e] ? s[nt][2 + e] * a.c : -INFINITY;
+                    float top = fmaxf(x0, x1);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float mn = fmaxf(m[nt][e], top);
+                    alpha[nt][e] = mn == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - mn);
+                    moved |= mn != m[nt][e];
+                    m[nt][e] = mn;
+                    const float ref = mn == -INFINITY ? 0.0f : mn;
+                    p[e] = exp2_fast(x0 - ref);
+                    p[2 + e] = exp2_fast(x1 - ref);
+                    l[nt][e] = l[nt][e] * alpha[nt][e] + (p[e] + p[2 + e]);
+                }
+                pf[nt][0] = transpose8x8(pack2<T>(p[0], p[1]));
+                pf[nt][1] = transpose8x8(pack2<T>(p[2], p[3]));
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int mt = 0; mt < HD / 16; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[mt][nt][e] *= alpha[nt][e & 1];
+            }
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+                unsigned vf[4];
+                const int row = (lane & 7) + ((lane >> 4) << 3), chunk = mt * 2 + ((lane >> 3) & 1);
+                ldmatrix_x4_trans(vf, vt + row * ROW_BYTES + ((chunk ^ (row & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[mt][nt], vf, pf[nt][0], pf[nt][1]);
+            }
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+
+            // ---- the end of the item, or of the share ----
+            const bool item_done = cc.unit + 1 == cc.u.U;
+            if (item_done || cc.pos + 1 == last) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
+                const unsigned long long item_end = item_begin + (unsigned)cc.u.U;
+                const long long all_rows = (long long)cc.u.s.n * a.group;
+                if (item_begin >= first && item_end <= last) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const long long r = (long long)cc.tile * TR + nt * 8 + (lane & 3) * 2 + e;
+                            if (r >= all_rows) continue;
+                            const float inv = l[nt][e] == 0.0f ? 0.0f : 1.0f / l[nt][e];
+                            T *dst = static_cast<T *>(a.out) + (long long)(cc.u.s.q0 + (int)((unsigned)r / (unsigned)a.group)) * a.out_token +
+                                     (long long)(cc.head * a.group + (int)((unsigned)r % (unsigned)a.group)) * a.out_head + (lane >> 2);
+#pragma unroll
+                            for (int mt = 0; mt < HD / 16; ++mt) {
+                                dst[mt * 16] = from_f32<T>(o[mt][nt][e] * inv);
+                                dst[mt * 16 + 8] = from_f32<T>(o[mt][nt][2 + e] * inv);
+                            }
+                        }
+                } else {
+                    // the first part if the share begins inside the item, otherwise the last: by then the ring is drained
+                    const int which = item_begin < first ? 0 : 1;
+                    if (which == 1) {
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        __syncwarp();
+                    }
+                    store_part(which, cc, o, m, l);
+                    if (lane == 0)
+                        heads[2 * warp + which] = PartHead{item_begin, item_end, cc.u.s.q0, (int)all_rows, cc.tile * TR, cc.head};
+                }
+                fresh = true;
+            }
+            advance<TR>(a, cc);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncthreads();
+
+    // ---- parts of one item within the CTA are joined; what began before it or goes on behind it becomes a record ----
+    const unsigned long long cta_first = share_begin(total, blockIdx.x * WARPS, shares);
+    const unsigned long long cta_last = share_begin(total, (blockIdx.x + 1) * WARPS, shares);
+    PartNote *note = static_cast<PartNote *>(a.ws) + blockIdx.x;
+    float *out_rec = part_records(a.ws, gridDim.x) + (size_t)blockIdx.x * 2 * REC;
+    if (threadIdx.x == 0) note->end = 0;
+    __syncthreads();
+    auto rec_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float *>(smem + (i >> 1) * STAGES * STAGE) : recs + (i >> 1) * REC; };
+    for (int i = 0; i < 2 * WARPS;) {
+        if (heads[i].end == 0) { ++i; continue; }
+        const PartHead h = heads[i];
+        int j = i + 1;  // records [i, j) are of this item
+        for (int k = i + 1; k < 2 * WARPS; ++k)
+            if (heads[k].end != 0) {
+                if (heads[k].begin != h.begin) break;
+                j = k + 1;
+            }
+        const bool whole = h.begin >= cta_first && h.end <= cta_last;
+        const int which = h.begin < cta_first ? 0 : 1;
+        const int rows = min(h.rows - h.tile_row, TR);
+        for (int row = warp; row < rows; row += WARPS) {
+            float mm = -INFINITY;
+            for (int k = i; k < j; ++k)
+                if (heads[k].end) mm = fmaxf(mm, rec_at(k)[TR * HD + row]);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            float ll = 0.0f, acc[HD / 32];
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) acc[e] = 0.0f;
+            for (int k = i; k < j; ++k)
+                if (heads[k].end) {
+                    const float *rec = rec_at(k);
+                    const float w = exp2_fast(rec[TR * HD + row] - ref);
+                    ll += w * rec[TR * HD + TR + row];
+#pragma unroll
+                    for (int e = 0; e < HD / 32; ++e) acc[e] += w * rec[row * HD + e * 32 + lane];
+                }
+            if (whole) {
+                const unsigned r = (unsigned)(h.tile_row + row);
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+                T *dst = static_cast<T *>(a.out) + (long long)(h.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
+                         (long long)(h.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
+#pragma unroll
+                for (int e = 0; e < HD / 32; ++e) dst[e * 32 + lane] = from_f32<T>(acc[e] * inv);
+            } else {
+                float *rec = out_rec + which * REC;
+#pragma unroll
+                for (int e = 0; e < HD / 32; ++e) rec[row * HD + e * 32 + lane] = acc[e];
+                if (lane == 0) {
+                    rec[TR * HD + row] = mm;
+                    rec[TR * HD + TR + row] = ll;
+                }
+            }
+        }
+        if (!whole && which == 1 && threadIdx.x == 0)
+            *note = PartNote{h.begin, h.end, total, h.q0, h.rows, h.tile_row, h.head};
+        i = j;
+    }
+}
+
+// Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
+// of the CTAs behind it.  A CTA per (note, row); SLICES groups of HD threads share the records.
+template <typename T, int HD>
+__global__ void __launch_bounds__(512) paged_merge_kernel(const PagedArgs a, int TR, int shares_per_part) {
+    constexpr int SLICES = 512 / HD;
+    __shared__ float sm[SLICES], sl[SLICES], so[SLICES][HD];
+    dependent_begin();
+    const PartNote n = static_cast<const PartNote *>(a.ws)[blockIdx.x];
+    const int row = blockIdx.y;
+    if (n.end == 0 || row >= min(n.rows - n.tile_row, TR)) return;
+    const int slice = threadIdx.x / HD, col = threadIdx.x % HD;
+    const size_t rec_floats = part_record_floats(TR, HD);
+    const float *recs = part_records(a.ws, a.parts);
+    const unsigned shares = (unsigned)a.parts * shares_per_part;
+    // the first CTA whose share begins at or behind the item's end: all before it, from the note's on, have a part
+    int lo = blockIdx.x + 1, hi = a.parts;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (share_begin(n.total, (unsigned)mid * shares_per_part, shares) < n.end) lo = mid + 1;
+        else hi = mid;
+    }
+    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    for (int c = blockIdx.x + slice; c < lo; c += SLICES) {
+        if (c > (int)blockIdx.x && share_begin(n.total, (unsigned)c * shares_per_part, shares) ==
+                                       share_begin(n.total, (unsigned)(c + 1) * shares_per_part, shares))
+            continue;  // an empty share
+        const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
+        const float rm = rec[TR * HD + row], rl = rec[TR * HD + TR + row], ro = rec[row * HD + col];
+        const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
+        const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
+        l = l * w0 + rl * w1;
+        o = o * w0 + ro * w1;
+        m = mn;
+    }
+    so[slice][col] = o;
+    if (col == 0) { sm[slice] = m; sl[slice] = l; }
+    __syncthreads();
+    if (slice) return;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) mm = fmaxf(mm, sm[s]);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+        const float w = exp2_fast(sm[s] - ref);
+        ll += w * sl[s];
+        acc += w * so[s][col];
+    }
+    const unsigned r = (unsigned)(n.tile_row + row);
+    T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
+             (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
+    dst[col] = from_f32<T>(ll == 0.0f ? 0.0f : acc / ll);
+}
+
+template <int HD, int NT> struct StreamShape {
+    // eight warps of three (head_dim 64: six) units each hold 192 KB in flight; 16 rows need the room for their records
+    static constexpr int WARPS = NT == 1 ? 8 : 6, STAGES = 384 / HD;
+    static constexpr size_t SMEM = (size_t)WARPS * STAGES * 2 * UNIT * HD * 2 + (size_t)WARPS * 8 * NT * (HD + 2) * sizeof(float);
+};
+
+template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream_t st) {
+    using S = StreamShape<HD, NT>;
+    auto kern = paged_stream_kernel<T, HD, NT, S::WARPS, S::STAGES>;
+    XN_ENSURE_SMEM(kern, S::SMEM);
+    a.parts = sm_count();
+    if (int rc = launch_dependent(kern, dim3((unsigned)a.parts), dim3(S::WARPS * 32), S::SMEM, st, a)) return rc;
+    return launch_paged_merge(sizeof(T) == 2 && std::is_same<T, __half>::value ? XN_F16 : XN_BF16, HD, 8 * NT, S::WARPS, a, st);
+}
+
+}  // namespace
+
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int shares_per_part, const PagedArgs &a, cudaStream_t st) {
+    const dim3 grid((unsigned)a.parts, (unsigned)rows), block(512);
+    if (dt == XN_F16)
+        return head_dim == 64 ? launch_dependent(paged_merge_kernel<__half, 64>, grid, block, 0, st, a, rows, shares_per_part)
+                              : launch_dependent(paged_merge_kernel<__half, 128>, grid, block, 0, st, a, rows, shares_per_part);
+    return head_dim == 64 ? launch_dependent(paged_merge_kernel<__nv_bfloat16, 64>, grid, block, 0, st, a, rows, shares_per_part)
+                          : launch_dependent(paged_merge_kernel<__nv_bfloat16, 128>, grid, block, 0, st, a, rows, shares_per_part);
+}
+
+size_t paged_stream_workspace(int head_dim) { return part_bytes(sm_count(), 16, head_dim); }
+
+int launch_paged_stream(xn_dtype dt, int head_dim, int rows, PagedArgs &a, cudaStream_t st) {
+    const bool wide = rows > 8;
+    if (dt == XN_F16) {
+        if (head_dim == 64) return wide ? launch_stream<__half, 64, 2>(a, st) : launch_stream<__half, 64, 1>(a, st);
+        return wide ? launch_stream<__half, 128, 2>(a, st) : launch_stream<__half, 128, 1>(a, st);
+    }
+    if (head_dim == 64) return wide ? launch_stream<__nv_bfloat16, 64, 2>(a, st) : launch_stream<__nv_bfloat16, 64, 1>(a, st);
+    return wide ? launch_stream<__nv_bfloat16, 128, 2>(a, st) : launch_stream<__nv_bfloat16, 128, 1>(a, st);
+}
+
+}  // namespace xn

@@ -11,6 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -725,6 +726,209 @@ XN_BINDING(prefill_forward, 2) {  // PrefillStack (world 1, fused attention), x 
     return out;
 }
 
+// ---------------------------------------------------------------------------------------------
+// Rotary positions, the paged cache, sampling (xn_mm_rope, xn_mm_paged_append, xn_mm_attention_paged, xn_mm_sample).
+// Tensors of a device other than the current one run there, on that device's current stream.
+// ---------------------------------------------------------------------------------------------
+xn_dtype float_code(const char *name, const at::Tensor &t) {
+    if (t.scalar_type() == at::kFloat) return XN_F32;
+    if (t.scalar_type() == at::kHalf) return XN_F16;
+    if (t.scalar_type() == at::kBFloat16) return XN_BF16;
+    raise_xn(XN_ERR_UNSUPPORTED, "%s not supported for dtype %s", name, dtype_name(t.scalar_type()));
+}
+
+// A tensor of the call beside `with`: on its device, of this type and shape (-1: any size).
+void want(const char *name, const char *what, const at::Tensor &t, const at::Tensor &with, at::ScalarType dt, at::IntArrayRef shape) {
+    bool fits = t.device() == with.device() && t.scalar_type() == dt && t.dim() == (int64_t)shape.size();
+    for (size_t i = 0; fits && i < shape.size(); ++i) fits = shape[i] < 0 || t.size((int64_t)i) == shape[i];
+    if (fits) return;
+    std::string s = "[";
+    for (size_t i = 0; i < shape.size(); ++i) s += (i ? ", " : "") + (shape[i] < 0 ? std::string("any") : std::to_string(shape[i]));
+    raise_xn(XN_ERR_INVALID, "%s: %s should be %s] of %s on %s, got %s of %s on %s", name, what, s.c_str(), dtype_name(dt),
+             with.device().str().c_str(), shape_text(t).c_str(), dtype_name(t.scalar_type()), t.device().str().c_str());
+}
+
+// What is written must have contiguous rows and no element twice.
+void want_output(const char *name, const char *what, const at::Tensor &t) {
+    bool fits = t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) <= 1;
+    for (int64_t i = 0; fits && i < t.dim(); ++i) fits = t.size(i) <= 1 || t.stride(i) != 0;
+    if (!fits) raise_xn(XN_ERR_INVALID, "%s: %s needs contiguous rows and no broadcast dimension", name, what);
+}
+
+at::Tensor rows_contiguous(const at::Tensor &t) { return t.dim() && t.stride(-1) == 1 ? t : t.contiguous(); }
+
+int flag(PyObject *o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised();
+    return v;
+}
+
+XN_BINDING(rope, 5) {  // x [tokens, heads, head_dim], positions, freqs, interleaved, out or None
+    const at::Tensor &x = tensor(a[0]);
+    const xn_dtype dt = float_code("rope", x);
+    if (x.dim() != 3) raise_xn(XN_ERR_INVALID, "rope expects [tokens, heads, head_dim], got %s", shape_text(x).c_str());
+    const at::Tensor &pos = tensor(a[1]), &freqs = tensor(a[2]);
+    want("rope", "positions", pos, x, at::kLong, {x.size(0)});
+    want("rope", "freqs", freqs, x, at::kDouble, {-1});
+    const int inter = flag(a[3]);
+    const at::Tensor *given = maybe_tensor(a[4]);
+    if (given) {
+        want("rope", "out", *given, x, x.scalar_type(), x.sizes());
+        want_output("rope", "out", *given);
+    }
+    if (x.size(2) % 2 || 2 * freqs.numel() > x.size(2))
+        raise_xn(XN_ERR_INVALID, "rope: %lld frequencies for heads of %lld elements", (long long)freqs.numel(), (long long)x.size(2));
+    require_cuda(x);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = given ? *given : empty(x.sizes(), x.scalar_type(), x.device());
+    const at::Tensor xc = rows_contiguous(x), pc = pos.contiguous(), fc = freqs.contiguous();
+    void *o = out.data_ptr(), *st = stream();
+    const void *xp = xc.data_ptr();
+    const int64_t *pp = (const int64_t *)pc.data_ptr();
+    const double *fp = (const double *)fc.data_ptr();
+    const size_t ot = (size_t)out.stride(0), oh = (size_t)out.stride(1), xt = (size_t)xc.stride(0), xh = (size_t)xc.stride(1);
+    const size_t tokens = (size_t)x.size(0), heads = (size_t)x.size(1), hd = (size_t)x.size(2), rot = 2 * (size_t)freqs.numel();
+    XN_CALL(xn_mm_rope(dt, o, ot, oh, xp, xt, xh, pp, fp, tokens, heads, hd, rot, inter, st));
+    return wrap(std::move(out));
+}
+
+void want_pools(const char *name, const at::Tensor &k, const at::Tensor &v) {
+    if (k.dim() != 4)
+        raise_xn(XN_ERR_INVALID, "%s expects pools of [pages, kv_heads, page_size, head_dim], got %s", name, shape_text(k).c_str());
+    want(name, "v_pages", v, k, k.scalar_type(), k.sizes());
+    if (k.strides() != v.strides()) raise_xn(XN_ERR_INVALID, "%s: k_pages and v_pages must have the same strides", name);
+    if (k.stride(3) != 1 && k.size(3) > 1) raise_xn(XN_ERR_INVALID, "%s: the pools' last dimension must be contiguous", name);
+}
+
+XN_BINDING(paged_append_, 9) {  // k_pages, v_pages, k, v, slots, q or None, positions or None, freqs or None, interleaved
+    const char *name = "paged_append_";
+    const at::Tensor &kp = tensor(a[0]), &vp = tensor(a[1]), &k = tensor(a[2]), &v = tensor(a[3]), &slots = tensor(a[4]);
+    const at::Tensor *q = maybe_tensor(a[5]), *pos = maybe_tensor(a[6]), *freqs = maybe_tensor(a[7]);
+    const int inter = flag(a[8]);
+    want_pools(name, kp, vp);
+    want_output(name, "the pools", kp);
+    const xn_dtype dt = float_code(name, kp);
+    const int64_t kv = kp.size(1), hd = kp.size(3);
+    if (k.dim() != 3) raise_xn(XN_ERR_INVALID, "%s expects k of [tokens, kv_heads, head_dim], got %s", name, shape_text(k).c_str());
+    const int64_t tokens = k.size(0);
+    want(name, "k", k, kp, kp.scalar_type(), {tokens, kv, hd});
+    want(name, "v", v, kp, kp.scalar_type(), {tokens, kv, hd});
+    want(name, "slots", slots, kp, at::kLong, {tokens});
+    if (q) want(name, "q", *q, kp, kp.scalar_type(), {tokens, -1, hd});
+    if (freqs) {
+        want(name, "freqs", *freqs, kp, at::kDouble, {-1});
+        if (!pos) raise_xn(XN_ERR_INVALID, "%s: freqs need positions", name);
+        want(name, "positions", *pos, kp, at::kLong, {tokens});
+    } else if (pos) {
+        raise_xn(XN_ERR_INVALID, "%s: positions need freqs", name);
+    }
+    if (hd % 2 || (freqs && 2 * freqs->numel() > hd))
+        raise_xn(XN_ERR_INVALID, "%s: %lld frequencies for heads of %lld elements", name, freqs ? (long long)freqs->numel() : 0ll, (long long)hd);
+    require_cuda(kp);
+    c10::cuda::CUDAGuard guard(kp.device());
+    const at::Tensor kc = rows_contiguous(k), vc = rows_contiguous(v), sc = slots.contiguous();
+    at::Tensor qc, pc, fc, out;
+    if (q) {
+        qc = rows_contiguous(*q);
+        out = empty(q->sizes(), q->scalar_type(), q->device());
+    }
+    if (freqs) {
+        pc = pos->contiguous();
+        fc = freqs->contiguous();
+    }
+    void *kpp = kp.data_ptr(), *vpp = vp.data_ptr(), *op = q ? out.data_ptr() : nullptr, *st = stream();
+    const void *kd = kc.data_ptr(), *vd = vc.data_ptr(), *qd = q ? qc.data_ptr() : nullptr;
+    const int64_t *sp = (const int64_t *)sc.data_ptr(), *pp = freqs ? (const int64_t *)pc.data_ptr() : nullptr;
+    const double *fp = freqs && freqs->numel() ? (const double *)fc.data_ptr() : nullptr;
+    const size_t qt = q ? (size_t)qc.stride(0) : 0, qh = q ? (size_t)qc.stride(1) : 0, heads = q ? (size_t)q->size(1) : 0;
+    const size_t rot = fp ? 2 * (size_t)freqs->numel() : 0;
+    XN_CALL(xn_mm_paged_append(dt, kpp, vpp, (size_t)kp.stride(0), (size_t)kp.stride(1), (size_t)kp.stride(2), (size_t)kp.size(0),
+                               (size_t)kp.size(2), kd, (size_t)kc.stride(0), (size_t)kc.stride(1), vd, (size_t)vc.stride(0),
+                               (size_t)vc.stride(1), sp, (size_t)tokens, (size_t)kv, (size_t)hd, op, qd, qt, qh, heads, pp, fp, rot, inter,
+                               st));
+    if (!q) Py_RETURN_NONE;
+    return wrap(std::move(out));
+}
+
+XN_BINDING(attention_paged, 10) {  // q, k_pages, v_pages, page_table, context, scale, query_starts, max_query, window, out (or None)
+    const char *name = "attention_paged";
+    const at::Tensor &q = tensor(a[0]), &kp = tensor(a[1]), &vp = tensor(a[2]), &table = tensor(a[3]), &context = tensor(a[4]);
+    const float scale = (float)float_arg(a[5]);
+    const at::Tensor *starts = maybe_tensor(a[6]), *given = maybe_tensor(a[9]);
+    const size_t max_query = a[7] == Py_None ? 0 : size_arg(a[7]), window = size_arg(a[8]);
+    if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16)
+        raise_xn(XN_ERR_UNSUPPORTED, "%s not supported for dtype %s", name, dtype_name(q.scalar_type()));
+    if (q.dim() != 3) raise_xn(XN_ERR_INVALID, "%s expects q of [tokens, heads, head_dim], got %s", name, shape_text(q).c_str());
+    want_pools(name, kp, vp);
+    want(name, "k_pages", kp, q, q.scalar_type(), {-1, -1, -1, q.size(2)});
+    want(name, "page_table", table, q, at::kInt, {-1, -1});
+    const int64_t batch = table.size(0);
+    want(name, "context", context, q, at::kInt, {batch});
+    if (starts) want(name, "query_starts", *starts, q, at::kInt, {batch + 1});
+    if (given) {
+        want(name, "out", *given, q, q.scalar_type(), q.sizes());
+        want_output(name, "out", *given);
+    }
+    const int64_t kv = kp.size(1), hd = q.size(2);
+    if (hd != 64 && hd != 128) raise_xn(XN_ERR_INVALID, "%s: head_dim %lld is not supported (64 and 128 are)", name, (long long)hd);
+    if (kv ? q.size(1) % kv != 0 : q.size(1) != 0)
+        raise_xn(XN_ERR_INVALID, "%s: %lld query heads do not share %lld key heads evenly", name, (long long)q.size(1), (long long)kv);
+    if (!starts && batch != q.size(0))
+        raise_xn(XN_ERR_INVALID, "%s: %lld rows for %lld sequences of one row each", name, (long long)q.size(0), (long long)batch);
+    require_cuda(q);
+    c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = given ? *given : empty(q.sizes(), q.scalar_type(), q.device());
+    at::Tensor qc = rows_contiguous(q);
+    if (qc.stride(0) % 8 || qc.stride(1) % 8 || (uintptr_t)qc.data_ptr() % 16) qc = qc.clone(at::MemoryFormat::Contiguous);
+    const at::Tensor tc = rows_contiguous(table), cc = context.contiguous();
+    at::Tensor sc;
+    if (starts) sc = starts->contiguous();
+    const size_t ws_bytes = xn_mm_attention_paged_workspace_bytes((size_t)q.size(2));
+    at::Tensor ws = empty({(int64_t)ws_bytes}, at::kByte, q.device());
+    void *o = out.data_ptr(), *w = ws.data_ptr(), *st = stream();
+    const void *qd = qc.data_ptr(), *kd = kp.data_ptr(), *vd = vp.data_ptr();
+    const int32_t *td = (const int32_t *)tc.data_ptr(), *cd = (const int32_t *)cc.data_ptr(),
+                  *sd = starts ? (const int32_t *)sc.data_ptr() : nullptr;
+    const xn_dtype dt = q.scalar_type() == at::kHalf ? XN_F16 : XN_BF16;
+    XN_CALL(xn_mm_attention_paged(dt, o, (size_t)out.stride(0), (size_t)out.stride(1), qd, (size_t)qc.stride(0), (size_t)qc.stride(1),
+                                  (size_t)q.size(0), (size_t)q.size(1), kd, vd, (size_t)kp.stride(0), (size_t)kp.stride(1),
+                                  (size_t)kp.stride(2), (size_t)kp.size(0), (size_t)kp.size(2), (size_t)kp.size(1), (size_t)q.size(2),
+                                  td, (size_t)tc.stride(0), (size_t)table.size(1), cd, sd, (size_t)batch, max_query, window, scale, w,
+                                  ws_bytes, st));
+    return wrap(std::move(out));
+}
+
+XN_BINDING(sample, 6) {  // logits [rows, vocab], uniform, temperature, top_k, top_p, min_p (or None)
+    const char *name = "sample";
+    const at::Tensor &x = tensor(a[0]), &u = tensor(a[1]);
+    const at::Tensor *setting[4];
+    const xn_dtype dt = float_code(name, x);
+    if (x.dim() != 2) raise_xn(XN_ERR_INVALID, "sample expects [rows, vocabulary], got %s", shape_text(x).c_str());
+    const int64_t rows = x.size(0);
+    want(name, "uniform", u, x, at::kFloat, {rows});
+    static const char *const NAMES[4] = {"temperature", "top_k", "top_p", "min_p"};
+    for (int i = 0; i < 4; ++i)
+        if ((setting[i] = maybe_tensor(a[2 + i]))) want(name, NAMES[i], *setting[i], x, i == 1 ? at::kInt : at::kFloat, {rows});
+    if (rows && x.size(1) == 0) raise_xn(XN_ERR_INVALID, "sample: an empty vocabulary");
+    require_cuda(x);
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor out = empty({rows}, at::kLong, x.device());
+    const at::Tensor xc = rows_contiguous(x), uc = u.contiguous();
+    at::Tensor kept[4];
+    const void *sp[4];
+    for (int i = 0; i < 4; ++i) {
+        if (setting[i]) kept[i] = setting[i]->contiguous();
+        sp[i] = setting[i] ? kept[i].data_ptr() : nullptr;
+    }
+    int64_t *o = (int64_t *)out.data_ptr();
+    const void *xp = xc.data_ptr();
+    const float *up = (const float *)uc.data_ptr();
+    void *st = stream();
+    XN_CALL(xn_mm_sample(dt, o, xp, (size_t)xc.stride(0), (size_t)rows, (size_t)x.size(1), up, (const float *)sp[0], (const int32_t *)sp[1],
+                         (const float *)sp[2], (const float *)sp[3], st));
+    return wrap(std::move(out));
+}
+
 XN_BINDING(set_error_class, 1) {
     Py_INCREF(a[0]);
     Py_XDECREF(g_error_class);
@@ -737,7 +941,8 @@ PyMethodDef METHODS[] = {
     XN_METHOD(matmul_), XN_METHOD(matmul_with_t), XN_METHOD(linear), XN_METHOD(quantize_rows_i8), XN_METHOD(linear_block),
     XN_METHOD(linear_q4_forward), XN_METHOD(split_rows_e4m3), XN_METHOD(linear_fp8), XN_METHOD(rms_norm), XN_METHOD(softmax),
     XN_METHOD(silu_mul), XN_METHOD(add), XN_METHOD(conv1d), XN_METHOD(conv_transpose1d), XN_METHOD(decoder_step),
-    XN_METHOD(prefill_forward), XN_METHOD(set_error_class), {nullptr, nullptr, 0, nullptr}};
+    XN_METHOD(prefill_forward), XN_METHOD(rope), XN_METHOD(paged_append_), XN_METHOD(attention_paged), XN_METHOD(sample),
+    XN_METHOD(set_error_class), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_host", "Native host path of the operators.", -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,86 @@
+// What the kernels of attention over a paged cache share: the call's arguments, the geometry of a sequence, and the records of
+// rows whose keys were shared out.
+#pragma once
+#include "common.cuh"
+
+namespace xn {
+
+// Sequence b has the query rows [starts[b], starts[b + 1]) (starts == null: row b alone) and context[b] keys, its own rows'
+// keys the last of them; key j lies in row j % page_size of page table[b][j / page_size].  Row i of n sees the keys
+// j <= i + context - n, of those the last `window` only (0: all).  Lengths and indexes come from device memory and are
+// bounded where they are read: nothing they say can lead outside the tensors.  A page index outside the pool reads as a
+// page of zeros.
+struct PagedArgs {
+    const void *q, *k, *v;
+    void *out;
+    const int *table, *context, *starts;
+    long long q_token, q_head, out_token, out_head;   // strides in elements
+    long long page_stride, head_stride, row_stride;   // of both pools
+    long long table_stride;
+    int tokens, batch, heads, kv_heads, group;
+    int num_pages, page_size, page_shift, max_pages;  // page_shift: log2(page_size), or -1
+    int window;
+    float c;  // scale * log2(e)
+    void *ws;
+    int parts;  // CTAs that share the work
+};
+
+struct Sequence {
+    int q0, n;    // first query row, number of them
+    int ctx, off; // keys, and the last key that row 0 sees
+};
+__device__ __forceinline__ Sequence load_sequence(const PagedArgs &a, int b) {
+    Sequence s;
+    if (a.starts) {
+        s.q0 = min(max(a.starts[b], 0), a.tokens);
+        s.n = min(max(a.starts[b + 1], s.q0), a.tokens) - s.q0;
+    } else {
+        s.q0 = min(b, a.tokens);
+        s.n = b < a.tokens ? 1 : 0;
+    }
+    const long long room = (long long)a.max_pages * a.page_size;
+    s.ctx = (int)min((long long)max(a.context[b], 0), room);
+    s.off = s.ctx - s.n;
+    return s;
+}
+
+// A row's result over a part of its keys: the sum of p v (head_dim floats), the maximum m of its scaled scores and the sum l of
+// p = 2^(score - m).  CTA c of `parts` writes the part that it did not begin into record 0 and the part that it does not end
+// into record 1, and leaves a note of the latter.
+struct PartNote {
+    unsigned long long begin, end, total;  // the item's units, and all units of the call; end == 0: no note
+    int q0, rows, tile_row, head;          // first query row of its sequence, rows of the sequence, first row of the item, kv head
+};
+__host__ __device__ constexpr size_t part_record_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
+__host__ __device__ constexpr size_t part_bytes(int parts, int rows, int hd) {
+    return ((size_t)parts * sizeof(PartNote) + 255) / 256 * 256 + (size_t)parts * 2 * part_record_floats(rows, hd) * sizeof(float);
+}
+__host__ __device__ inline float *part_records(void *ws, int parts) {
+    return reinterpret_cast<float *>(static_cast<char *>(ws) + ((size_t)parts * sizeof(PartNote) + 255) / 256 * 256);
+}
+// Units are dealt out evenly, in order: share g of `shares` gets [share_begin(g), share_begin(g + 1)).
+__host__ __device__ __forceinline__ unsigned long long share_begin(unsigned long long total, unsigned g, unsigned shares) {
+    return total / shares * g + total % shares * g / shares;
+}
+
+template <typename T> __device__ __forceinline__ unsigned pack2(float x, float y);
+template <> __device__ __forceinline__ unsigned pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // relative error about 2^-22; 0 for -inf
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// attention_paged_stream.cu: up to 16 rows of a key head at a time, any page size
+int launch_paged_stream(xn_dtype dt, int head_dim, int rows, PagedArgs &a, cudaStream_t st);
+size_t paged_stream_workspace(int head_dim);
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int shares_per_part, const PagedArgs &a, cudaStream_t st);
+
+}  // namespace xn

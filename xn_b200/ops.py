@@ -12,6 +12,7 @@ per token go through the native host module (csrc/host/binding.cpp); the rest bi
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -286,3 +287,70 @@ def silu_mul(x: torch.Tensor) -> torch.Tensor:
 
 def add(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return _host.add(a, b)
+
+
+# ---------------------------------------------------------------------------------------------
+# A serving step around the linears: rotary positions, a cache of pages, attention over it, the next token.
+# ---------------------------------------------------------------------------------------------
+def rope_frequencies(rotated: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, context: int = 4096,
+                     low_turns: float = 1.0, high_turns: float = 4.0, device=None) -> torch.Tensor:
+    """Radians per position of the ``rotated // 2`` pairs of a head, f64: ``base ** (-2 i / rotated)``, scaled for contexts
+    ``factor`` times as long as the ``context`` a model was trained on.  scaling: "none"; "linear" -- all divided by the
+    factor; "base" -- a larger base, which divides the slowest pair by the factor and leaves the fastest; "bands" --
+    pairs of fewer than ``low_turns`` turns over the trained context divided by it, those of more than ``high_turns`` left, a ramp
+    between them."""
+    if rotated <= 0 or rotated % 2:
+        raise XnError(_lib.ERR_INVALID, f"rope_frequencies: {rotated} rotated elements, an even number is wanted")
+    if scaling not in ("none", "linear", "base", "bands"):
+        raise XnError(_lib.ERR_INVALID, f"rope_frequencies: unknown scaling {scaling!r}")
+    if not (base > 0 and factor > 0 and context > 0 and 0 <= low_turns < high_turns):
+        raise XnError(_lib.ERR_INVALID, "rope_frequencies: base, factor and context are positive, low_turns below high_turns")
+    i = torch.arange(rotated // 2, dtype=torch.float64)
+    if scaling == "base":
+        base = base * factor ** (rotated / (rotated - 2)) if rotated > 2 else base
+    f = float(base) ** (-2.0 * i / rotated)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "bands":
+        keep = ((context * f / (2.0 * math.pi) - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    return f.to(device) if device is not None else f
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False,
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [tokens, heads, head_dim] (any strides) with the first ``2 len(freqs)`` elements of each head turned by their token's
+    position (int64 [tokens]): pairs side by side (``interleaved``: the reference's rope_i) or half the rotated part apart (rope).
+    freqs: f64, see rope_frequencies.  The angle is formed in 64 bits.  ``out`` may be x itself."""
+    return _host.rope(x, positions, freqs, interleaved, out)
+
+
+def paged_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
+                  q: torch.Tensor | None = None, positions: torch.Tensor | None = None, freqs: torch.Tensor | None = None,
+                  interleaved: bool = False) -> torch.Tensor | None:
+    """The new tokens of a batch into a paged cache, in one launch: k, v [tokens, kv_heads, head_dim] (views of the fused
+    projection) to their slots (int64 [tokens], page * page_size + row, distinct; one outside the pool stores nothing) of
+    k_pages, v_pages [pages, kv_heads, page_size, head_dim].  With freqs and positions, k is turned on the way as rope does.  Where
+    q [tokens, heads, head_dim] is given, returns it turned the same way (contiguous)."""
+    return _host.paged_append_(k_pages, v_pages, k, v, slots, q, positions, freqs, interleaved)
+
+
+def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, context: torch.Tensor,
+                    scale: float, query_starts: torch.Tensor | None = None, max_query: int | None = None, window: int = 0,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the newest tokens of a batch of sequences over a paged cache that already holds them
+    (xn_mm_attention_paged).  q [tokens, heads, head_dim]: the sequences' rows one after another, query_starts int32 [batch + 1] saying
+    where each begins (None: one row each); context int32 [batch]: keys of each with the new ones; page_table int32 [batch, pages].
+    Query heads share the pools' kv_heads evenly.  Row i of n sees key j iff j <= i + context - n, with a window > 0 only the last
+    `window` of those; a row that sees nothing is zeros.  Rows behind the last sequence are not written.  max_query: the longest
+    sequence's rows where the program knows it (the tensors are on the device); it decides which kernel runs, not what it
+    gives.  f16 / bf16, head_dim 64 or 128, any page size."""
+    return _host.attention_paged(q, k_pages, v_pages, page_table, context, scale, query_starts, max_query, window, out)
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+           top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None) -> torch.Tensor:
+    """The next token (int64) of every row of logits [rows, vocabulary], from uniform [rows] in [0, 1) (xn_mm_sample): the rows'
+    temperature (f32 [rows]; not positive: the largest logit), top_k (int32; 0: off), top_p (f32; 1: off) and min_p (f32; 0: off), in this order.
+    The draw walks the kept tokens in order of index; sums are exact, so equal inputs give equal tokens."""
+    return _host.sample(logits, uniform, temperature, top_k, top_p, min_p)
