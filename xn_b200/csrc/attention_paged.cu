@@ -1,10 +1,14 @@
 // Entry points of attention over a paged cache: checks, and which kernel a call gets.
+#include <math.h>
+
 #include "paged.cuh"
 
 using namespace xn;
 
 extern "C" size_t xn_mm_attention_paged_workspace_bytes(size_t head_dim) {
-    return head_dim == 64 || head_dim == 128 ? paged_stream_workspace((int)head_dim) : 0;
+    if (head_dim != 64 && head_dim != 128) return 0;
+    const size_t a = paged_stream_workspace((int)head_dim), b = paged_tc_workspace((int)head_dim);
+    return a > b ? a : b;
 }
 
 extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token_stride, size_t out_head_stride, const void *q,
@@ -49,10 +53,11 @@ extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token
     if ((page_size & (page_size - 1)) == 0)
         for (a.page_shift = 0; (size_t)1 << a.page_shift < page_size; ++a.page_shift) {}
     a.window = (int)(window < 0x3fffffffull ? window : 0x3fffffffull);
-    a.c = scale * 1.4426950408889634f;
+    a.c = fmaxf(scale * 1.4426950408889634f, 1e-37f);  // above zero: a masked score, -inf, stays -inf
     a.ws = workspace;
     if (!query_starts_or_null) max_query = 1;
     if (max_query > tokens || max_query == 0) max_query = tokens;
     const size_t rows = max_query * (heads / kv_heads);
+    if (rows > 16 && paged_tc_fits(a)) return launch_paged_tc(dtype, (int)head_dim, a, (cudaStream_t)stream);
     return launch_paged_stream(dtype, (int)head_dim, rows > 16 ? 16 : (int)rows, a, (cudaStream_t)stream);
 }

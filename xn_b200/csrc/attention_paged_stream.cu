@@ -435,64 +435,72 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
             }
         }
         if (!whole && which == 1 && threadIdx.x == 0)
-            *note = PartNote{h.begin, h.end, total, h.q0, h.rows, h.tile_row, h.head};
+            *note = PartNote{h.begin, h.end, total, h.q0, h.rows, h.tile_row, h.head, 1};
         i = j;
     }
 }
 
 // Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
-// of the CTAs behind it.  A CTA per (note, row); SLICES groups of HD threads share the records.
-template <typename T, int HD>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const PagedArgs a, int TR, int shares_per_part) {
-    constexpr int SLICES = 512 / HD;
-    __shared__ float sm[SLICES], sl[SLICES], so[SLICES][HD];
+// of the CTAs behind it.  A block takes ROWS rows of a note's item; SLICES groups of HD threads share a row's records.
+template <typename T, int HD, int SLICES>
+__global__ void __launch_bounds__(512) paged_merge_kernel(const PagedArgs a, int rec_rows, int used, int shares_per_part) {
+    constexpr int ROWS = 512 / HD / SLICES;
+    __shared__ float sm[ROWS][SLICES], sl[ROWS][SLICES], so[ROWS][SLICES][HD];
     dependent_begin();
     const PartNote n = static_cast<const PartNote *>(a.ws)[blockIdx.x];
-    const int row = blockIdx.y;
-    if (n.end == 0 || row >= min(n.rows - n.tile_row, TR)) return;
-    const int slice = threadIdx.x / HD, col = threadIdx.x % HD;
-    const size_t rec_floats = part_record_floats(TR, HD);
+    if (n.end == 0) return;
+    const int in_block = threadIdx.x / (HD * SLICES), slice = threadIdx.x / HD % SLICES, col = threadIdx.x % HD;
+    const int row = blockIdx.y * ROWS + in_block;
+    const int item_row = (row >> 7) * used + (row & 127);
+    const bool real = row < rec_rows && (row & 127) < used && n.tile_row + item_row < n.rows;
+    const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
     const unsigned shares = (unsigned)a.parts * shares_per_part;
-    // the first CTA whose share begins at or behind the item's end: all before it, from the note's on, have a part
+    auto begin_of = [&](int c) { return share_begin(n.total, (unsigned)c * shares_per_part, shares); };
+    // the first CTA whose share begins at or behind the item's end: all before it, from the note's on, may have a part
     int lo = blockIdx.x + 1, hi = a.parts;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (share_begin(n.total, (unsigned)mid * shares_per_part, shares) < n.end) lo = mid + 1;
+        if (begin_of(mid) < n.end) lo = mid + 1;
         else hi = mid;
     }
     float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int c = blockIdx.x + slice; c < lo; c += SLICES) {
-        if (c > (int)blockIdx.x && share_begin(n.total, (unsigned)c * shares_per_part, shares) ==
-                                       share_begin(n.total, (unsigned)(c + 1) * shares_per_part, shares))
-            continue;  // an empty share
-        const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-        const float rm = rec[TR * HD + row], rl = rec[TR * HD + TR + row], ro = rec[row * HD + col];
-        const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
-        const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
-        l = l * w0 + rl * w1;
-        o = o * w0 + ro * w1;
-        m = mn;
-    }
-    so[slice][col] = o;
-    if (col == 0) { sm[slice] = m; sl[slice] = l; }
-    __syncthreads();
-    if (slice) return;
-    float mm = -INFINITY;
+    if (real)
+        for (int c = blockIdx.x + slice; c < lo; c += SLICES) {
+            if (c > (int)blockIdx.x) {  // whether a key block begins in its share
+                const unsigned long long from = begin_of(c) - n.begin, to = min(begin_of(c + 1), n.end) - n.begin;
+                if ((from + n.step - 1) / n.step >= (to + n.step - 1) / n.step) continue;
+            }
+            const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
+            const float rm = rec[rec_rows * HD + row], rl = rec[rec_rows * HD + rec_rows + row], ro = rec[(size_t)row * HD + col];
+            const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
+            const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
+            l = l * w0 + rl * w1;
+            o = o * w0 + ro * w1;
+            m = mn;
+        }
+    if (SLICES > 1) {
+        so[in_block][slice][col] = o;
+        if (col == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
+        __syncthreads();
+        if (slice) return;
+        float mm = -INFINITY;
 #pragma unroll
-    for (int s = 0; s < SLICES; ++s) mm = fmaxf(mm, sm[s]);
-    const float ref = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, acc = 0.0f;
+        for (int s = 0; s < SLICES; ++s) mm = fmaxf(mm, sm[in_block][s]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        l = o = 0.0f;
 #pragma unroll
-    for (int s = 0; s < SLICES; ++s) {
-        const float w = exp2_fast(sm[s] - ref);
-        ll += w * sl[s];
-        acc += w * so[s][col];
+        for (int s = 0; s < SLICES; ++s) {
+            const float w = exp2_fast(sm[in_block][s] - ref);
+            l += w * sl[in_block][s];
+            o += w * so[in_block][s][col];
+        }
     }
-    const unsigned r = (unsigned)(n.tile_row + row);
+    if (!real) return;
+    const unsigned r = (unsigned)(n.tile_row + item_row);
     T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
              (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-    dst[col] = from_f32<T>(ll == 0.0f ? 0.0f : acc / ll);
+    dst[col] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
 }
 
 template <int HD, int NT> struct StreamShape {
@@ -507,18 +515,26 @@ template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream
     XN_ENSURE_SMEM(kern, S::SMEM);
     a.parts = sm_count();
     if (int rc = launch_dependent(kern, dim3((unsigned)a.parts), dim3(S::WARPS * 32), S::SMEM, st, a)) return rc;
-    return launch_paged_merge(sizeof(T) == 2 && std::is_same<T, __half>::value ? XN_F16 : XN_BF16, HD, 8 * NT, S::WARPS, a, st);
+    return launch_paged_merge(FMT_OF<T>, HD, 8 * NT, 8 * NT, S::WARPS, a, st);
 }
 
 }  // namespace
 
-int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int shares_per_part, const PagedArgs &a, cudaStream_t st) {
-    const dim3 grid((unsigned)a.parts, (unsigned)rows), block(512);
-    if (dt == XN_F16)
-        return head_dim == 64 ? launch_dependent(paged_merge_kernel<__half, 64>, grid, block, 0, st, a, rows, shares_per_part)
-                              : launch_dependent(paged_merge_kernel<__half, 128>, grid, block, 0, st, a, rows, shares_per_part);
-    return head_dim == 64 ? launch_dependent(paged_merge_kernel<__nv_bfloat16, 64>, grid, block, 0, st, a, rows, shares_per_part)
-                          : launch_dependent(paged_merge_kernel<__nv_bfloat16, 128>, grid, block, 0, st, a, rows, shares_per_part);
+namespace {
+// Few rows may have a record from every CTA: all threads of a block share one row's.  Many rows have a few each.
+template <typename T, int HD> int launch_merge(int rows, int used, int shares, const PagedArgs &a, cudaStream_t st) {
+    if (rows <= 16)
+        return launch_dependent(paged_merge_kernel<T, HD, 512 / HD>, dim3((unsigned)a.parts, (unsigned)rows), dim3(512), 0, st, a, rows, used,
+                                shares);
+    constexpr int ROWS = 512 / HD;
+    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS - 1) / ROWS)), dim3(512), 0, st, a,
+                            rows, used, shares);
+}
+}  // namespace
+
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, int shares, const PagedArgs &a, cudaStream_t st) {
+    if (dt == XN_F16) return head_dim == 64 ? launch_merge<__half, 64>(rows, used, shares, a, st) : launch_merge<__half, 128>(rows, used, shares, a, st);
+    return head_dim == 64 ? launch_merge<__nv_bfloat16, 64>(rows, used, shares, a, st) : launch_merge<__nv_bfloat16, 128>(rows, used, shares, a, st);
 }
 
 size_t paged_stream_workspace(int head_dim) { return part_bytes(sm_count(), 16, head_dim); }

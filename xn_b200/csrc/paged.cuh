@@ -1,6 +1,8 @@
 // What the kernels of attention over a paged cache share: the call's arguments, the geometry of a sequence, and the records of
 // rows whose keys were shared out.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace xn {
@@ -50,6 +52,7 @@ __device__ __forceinline__ Sequence load_sequence(const PagedArgs &a, int b) {
 struct PartNote {
     unsigned long long begin, end, total;  // the item's units, and all units of the call; end == 0: no note
     int q0, rows, tile_row, head;          // first query row of its sequence, rows of the sequence, first row of the item, kv head
+    int step;                              // units per key block: a CTA holds the blocks that begin in its share
 };
 __host__ __device__ constexpr size_t part_record_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 __host__ __device__ constexpr size_t part_bytes(int parts, int rows, int hd) {
@@ -63,6 +66,7 @@ __host__ __device__ __forceinline__ unsigned long long share_begin(unsigned long
     return total / shares * g + total % shares * g / shares;
 }
 
+template <typename T> constexpr xn_dtype FMT_OF = std::is_same<T, __half>::value ? XN_F16 : XN_BF16;
 template <typename T> __device__ __forceinline__ unsigned pack2(float x, float y);
 template <> __device__ __forceinline__ unsigned pack2<__half>(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -81,6 +85,11 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error about 2
 // attention_paged_stream.cu: up to 16 rows of a key head at a time, any page size
 int launch_paged_stream(xn_dtype dt, int head_dim, int rows, PagedArgs &a, cudaStream_t st);
 size_t paged_stream_workspace(int head_dim);
-int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int shares_per_part, const PagedArgs &a, cudaStream_t st);
+// Records of `rows` rows, of which the first `used` of every 128 are rows of the item; a CTA of `a.parts` has `shares` shares.
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, int shares, const PagedArgs &a, cudaStream_t st);
+// attention_paged_tc.cu: 256 rows of a key head at a time on the tensor-memory MMAs; pages of a multiple of 8 rows
+bool paged_tc_fits(const PagedArgs &a);
+size_t paged_tc_workspace(int head_dim);
+int launch_paged_tc(xn_dtype dt, int head_dim, const PagedArgs &a, cudaStream_t st);
 
 }  // namespace xn

@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <initializer_list>
+
 #include "common.cuh"
 #include "wait.cuh"
 
@@ -155,5 +157,9 @@ int make_map3(CUtensorMap *map, const void *base, int elem, size_t rows, size_t 
 // [k, n] operand with n contiguous, 16-bit elements; box 64 n x 64 k.
 int make_map_mn(CUtensorMap *map, const void *base, size_t n, size_t k, size_t ld, size_t batch, size_t batch_stride,
                 int *batch_inner);
+// Rows of k 16-bit elements laid out over up to three further dimensions (sizes, strides in elements, box sizes, innermost first);
+// a box covers 64 elements of each row, 128-byte swizzle, out-of-range reads give zeros.
+int make_map_rows(CUtensorMap *map, const void *base, size_t k, std::initializer_list<size_t> sizes, std::initializer_list<size_t> strides,
+                  std::initializer_list<unsigned> box);
 
 }  // namespace xn

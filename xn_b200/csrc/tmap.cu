@@ -85,4 +85,23 @@ int make_map_mn(CUtensorMap *map, const void *base, size_t n, size_t k, size_t l
     return XN_OK;
 }
 
+int make_map_rows(CUtensorMap *map, const void *base, size_t k, std::initializer_list<size_t> sizes, std::initializer_list<size_t> strides,
+                  std::initializer_list<unsigned> box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(XN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[4] = {(cuuint64_t)k}, pitch[3] = {};
+    cuuint32_t boxes[4] = {64}, estr[4] = {1, 1, 1, 1};
+    int n = 1;
+    for (size_t v : sizes) dims[n++] = (cuuint64_t)v;
+    n = 0;
+    for (size_t v : strides) pitch[n++] = (cuuint64_t)v * 2;
+    n = 1;
+    for (unsigned v : box) boxes[n++] = v;
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)n, const_cast<void *>(base), dims, pitch, boxes, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(XN_ERR_CUDA, "cuTensorMapEncodeTiled (%d-D rows) failed with code %d", n, (int)r);
+    return XN_OK;
+}
+
 }  // namespace xn
