@@ -386,8 +386,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
     const unsigned long long cta_last = share_begin(total, (blockIdx.x + 1) * WARPS, shares);
     PartNote *note = static_cast<PartNote *>(a.ws) + blockIdx.x;
     float *out_rec = part_records(a.ws, gridDim.x) + (size_t)blockIdx.x * 2 * REC;
-    if (threadIdx.x == 0) note->end = 0;
-    __syncthreads();
+    PartNote said{};
     auto rec_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float *>(smem + (i >> 1) * STAGES * STAGE) : recs + (i >> 1) * REC; };
     for (int i = 0; i < 2 * WARPS;) {
         if (heads[i].end == 0) { ++i; continue; }
@@ -434,73 +433,66 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                 }
             }
         }
+        if (!whole && which == 0) said.joined = 1;
         if (!whole && which == 1 && threadIdx.x == 0)
-            *note = PartNote{h.begin, h.end, total, h.q0, h.rows, h.tile_row, h.head, 1};
+            said = PartNote{said.joined, (int)(share_of(h.end - 1, total, shares) / WARPS), h.q0, h.rows, h.tile_row, h.head};
         i = j;
     }
+    if (threadIdx.x == 0) *note = said;
 }
 
 // Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
-// of the CTAs behind it.  A block takes ROWS rows of a note's item; SLICES groups of HD threads share a row's records.
+// of the CTAs behind it.  A thread holds four columns of a row; SLICES groups of threads share a row's records.
+constexpr int MERGE_NT = 256;
 template <typename T, int HD, int SLICES>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const PagedArgs a, int rec_rows, int used, int shares_per_part) {
-    constexpr int ROWS = 512 / HD / SLICES;
-    __shared__ float sm[ROWS][SLICES], sl[ROWS][SLICES], so[ROWS][SLICES][HD];
+__global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
+    constexpr int LANES = HD / 4, ROWS = MERGE_NT / LANES / SLICES;
+    __shared__ float sm[ROWS][SLICES], sl[ROWS][SLICES];
+    __shared__ float4 so[ROWS][SLICES][LANES];
     dependent_begin();
-    const PartNote n = static_cast<const PartNote *>(a.ws)[blockIdx.x];
-    if (n.end == 0) return;
-    const int in_block = threadIdx.x / (HD * SLICES), slice = threadIdx.x / HD % SLICES, col = threadIdx.x % HD;
+    const PartNote *notes = static_cast<const PartNote *>(a.ws);
+    const PartNote n = notes[blockIdx.x];
+    if (n.last == 0) return;
+    const int in_block = threadIdx.x / (LANES * SLICES), slice = threadIdx.x / LANES % SLICES, lane = threadIdx.x % LANES;
     const int row = blockIdx.y * ROWS + in_block;
     const int item_row = (row >> 7) * used + (row & 127);
     const bool real = row < rec_rows && (row & 127) < used && n.tile_row + item_row < n.rows;
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
-    const unsigned shares = (unsigned)a.parts * shares_per_part;
-    auto begin_of = [&](int c) { return share_begin(n.total, (unsigned)c * shares_per_part, shares); };
-    // the first CTA whose share begins at or behind the item's end: all before it, from the note's on, may have a part
-    int lo = blockIdx.x + 1, hi = a.parts;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (begin_of(mid) < n.end) lo = mid + 1;
-        else hi = mid;
-    }
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    auto join = [&](float rm, float rl, const float4 &ro) {
+        const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
+        const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
+        l = l * w0 + rl * w1;
+        o.x = o.x * w0 + ro.x * w1;
+        o.y = o.y * w0 + ro.y * w1;
+        o.z = o.z * w0 + ro.z * w1;
+        o.w = o.w * w0 + ro.w * w1;
+        m = mn;
+    };
     if (real)
-        for (int c = blockIdx.x + slice; c < lo; c += SLICES) {
-            if (c > (int)blockIdx.x) {  // whether a key block begins in its share
-                const unsigned long long from = begin_of(c) - n.begin, to = min(begin_of(c + 1), n.end) - n.begin;
-                if ((from + n.step - 1) / n.step >= (to + n.step - 1) / n.step) continue;
-            }
+        for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
+            if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
             const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-            const float rm = rec[rec_rows * HD + row], rl = rec[rec_rows * HD + rec_rows + row], ro = rec[(size_t)row * HD + col];
-            const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
-            const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
-            l = l * w0 + rl * w1;
-            o = o * w0 + ro * w1;
-            m = mn;
+            join(rec[rec_rows * HD + row], rec[rec_rows * HD + rec_rows + row], reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane]);
         }
     if (SLICES > 1) {
-        so[in_block][slice][col] = o;
-        if (col == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
+        so[in_block][slice][lane] = o;
+        if (lane == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
         __syncthreads();
         if (slice) return;
-        float mm = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < SLICES; ++s) mm = fmaxf(mm, sm[in_block][s]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        l = o = 0.0f;
-#pragma unroll
-        for (int s = 0; s < SLICES; ++s) {
-            const float w = exp2_fast(sm[in_block][s] - ref);
-            l += w * sl[in_block][s];
-            o += w * so[in_block][s][col];
-        }
+        for (int s = 1; s < SLICES; ++s) join(sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
     }
     if (!real) return;
     const unsigned r = (unsigned)(n.tile_row + item_row);
     T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
              (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-    dst[col] = from_f32<T>(l == 0.0f ? 0.0f : o / l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint2 w;
+    w.x = pack2<T>(o.x * inv, o.y * inv);
+    w.y = pack2<T>(o.z * inv, o.w * inv);
+    reinterpret_cast<uint2 *>(dst)[lane] = w;
 }
 
 template <int HD, int NT> struct StreamShape {
@@ -515,26 +507,25 @@ template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream
     XN_ENSURE_SMEM(kern, S::SMEM);
     a.parts = sm_count();
     if (int rc = launch_dependent(kern, dim3((unsigned)a.parts), dim3(S::WARPS * 32), S::SMEM, st, a)) return rc;
-    return launch_paged_merge(FMT_OF<T>, HD, 8 * NT, 8 * NT, S::WARPS, a, st);
+    return launch_paged_merge(FMT_OF<T>, HD, 8 * NT, 8 * NT, a, st);
 }
 
 }  // namespace
 
 namespace {
 // Few rows may have a record from every CTA: all threads of a block share one row's.  Many rows have a few each.
-template <typename T, int HD> int launch_merge(int rows, int used, int shares, const PagedArgs &a, cudaStream_t st) {
+template <typename T, int HD> int launch_merge(int rows, int used, const PagedArgs &a, cudaStream_t st) {
+    constexpr int ROWS = MERGE_NT * 4 / HD;
     if (rows <= 16)
-        return launch_dependent(paged_merge_kernel<T, HD, 512 / HD>, dim3((unsigned)a.parts, (unsigned)rows), dim3(512), 0, st, a, rows, used,
-                                shares);
-    constexpr int ROWS = 512 / HD;
-    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS - 1) / ROWS)), dim3(512), 0, st, a,
-                            rows, used, shares);
+        return launch_dependent(paged_merge_kernel<T, HD, ROWS>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
+    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS - 1) / ROWS)), dim3(MERGE_NT), 0, st,
+                            a, rows, used);
 }
 }  // namespace
 
-int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, int shares, const PagedArgs &a, cudaStream_t st) {
-    if (dt == XN_F16) return head_dim == 64 ? launch_merge<__half, 64>(rows, used, shares, a, st) : launch_merge<__half, 128>(rows, used, shares, a, st);
-    return head_dim == 64 ? launch_merge<__nv_bfloat16, 64>(rows, used, shares, a, st) : launch_merge<__nv_bfloat16, 128>(rows, used, shares, a, st);
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, const PagedArgs &a, cudaStream_t st) {
+    if (dt == XN_F16) return head_dim == 64 ? launch_merge<__half, 64>(rows, used, a, st) : launch_merge<__half, 128>(rows, used, a, st);
+    return head_dim == 64 ? launch_merge<__nv_bfloat16, 64>(rows, used, a, st) : launch_merge<__nv_bfloat16, 128>(rows, used, a, st);
 }
 
 size_t paged_stream_workspace(int head_dim) { return part_bytes(sm_count(), 16, head_dim); }

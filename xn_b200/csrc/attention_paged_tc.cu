@@ -118,7 +118,7 @@ struct Walk {
 
 struct TcShared {
     uint64_t q_full, q_empty, k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty, red_full, red_empty, seg_full[SEGS], seg_empty[SEGS];
+    uint64_t s_full[2], p_full[2][2], o_full[2], o_empty, red_full, red_empty, seg_full[SEGS], seg_empty[SEGS];
     u64 scan[TC_WARPS], start_base, start_sum;
     Segment segs[SEGS];
     uint32_t tmem_slot;
@@ -182,7 +182,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         for (int i = 0; i < V_STAGES; ++i) { mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], 4);
+            mbar_init(&sh.p_full[i][0], 4);
+            mbar_init(&sh.p_full[i][1], 4);
             mbar_init(&sh.o_full[i], 1);
         }
         mbar_init(&sh.o_empty, 8);
@@ -371,7 +372,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     Segment g{};
                     u64 begin, end;
                     const bool more = walk.next(args, g, &begin, &end);
-                    if (more && g.record == 1) note = PartNote{begin, end, total, g.row0 - g.tok0, g.n * p.group, g.tok0 * p.group, g.head, 1 << g.dual};
+                    if (more && g.record == 0) note.joined = 1;
+                    if (more && g.record == 1)
+                        note = PartNote{note.joined, (int)share_of(end - 1, total, gridDim.x), g.row0 - g.tok0, g.n * p.group, g.tok0 * p.group, g.head};
                     if (!more) g.nb = 0;
                     const unsigned slot = n_seg % SEGS;
                     if (!mbar_wait(&sh.seg_empty[slot], ((n_seg / SEGS) & 1u) ^ 1u, args.wait)) break;
@@ -398,17 +401,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
                     umma_commit(&sh.s_full[t]);
                 };
-                auto product = [&](int t, unsigned stage, bool add) {  // O_t (+)= P_t V
+                auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
+                // O_t (+)= P_t V, the first 64 keys as soon as their probabilities are there
+                auto product = [&](int t, unsigned stage, bool add) -> bool {
                     const uint32_t db = smem_desc_mn(sV + stage * STAGE, HALF);
-    #pragma unroll
-                    for (int ks = 0; ks < KEYS / 16; ++ks)
-                        umma_from_tmem(tmem_base + 256 + t * HD, tmem_base + t * KEYS + ks * 8, db + ks * (uint32_t)(16 * BKB >> 4), IDESC_O,
-                                       add || ks != 0);
+                    const unsigned n = np[t]++;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!mbar_wait(&sh.p_full[t][half], n & 1u, args.wait)) return false;
+                        after();
+#pragma unroll
+                        for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+                            umma_from_tmem(tmem_base + 256 + t * HD, tmem_base + t * KEYS + ks * 8, db + ks * (uint32_t)(16 * BKB >> 4), IDESC_O,
+                                           add || ks != 0);
+                    }
+                    return true;
                 };
                 auto wait_k = [&](unsigned n) { return mbar_wait(&sh.k_full[n % K_STAGES], (n / K_STAGES) & 1u, args.wait); };
                 auto wait_v = [&](unsigned n) { return mbar_wait(&sh.v_full[n % V_STAGES], (n / V_STAGES) & 1u, args.wait); };
-                auto wait_p = [&](int t) { const unsigned n = np[t]++; return mbar_wait(&sh.p_full[t], n & 1u, args.wait); };
-                auto after = [] { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); };
                 for (unsigned n_seg = 0; ok; ++n_seg) {
                     const unsigned slot = n_seg % SEGS;
                     if (!mbar_wait(&sh.seg_full[slot], (n_seg / SEGS) & 1u, args.wait)) break;
@@ -428,10 +438,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             const bool more = j + 1 < nb;
                             for (int t = 0; t < 2 && ok; ++t) {
                                 // the first products of an item overwrite the accumulators: the rows before must have been read
-                                ok = wait_p(t) && (t || (wait_v(nv) && (j || mbar_wait(&sh.o_empty, o_phase, args.wait))));
+                                ok = (t || (wait_v(nv) && (j || mbar_wait(&sh.o_empty, o_phase, args.wait)))) && product(t, nv % V_STAGES, j != 0);
                                 if (!ok) break;
-                                after();
-                                product(t, nv % V_STAGES, j != 0);
                                 if (t) umma_commit(&sh.v_empty[nv % V_STAGES]);
                                 if (!more) umma_commit(&sh.o_full[t]);
                                 else {
@@ -460,10 +468,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         if (nb <= 2) umma_commit(&sh.q_empty);
                         for (int j = 0; j < nb && ok; ++j, ++nv) {
                             const int t = j & 1;
-                            ok = wait_p(t) && wait_v(nv) && (j || mbar_wait(&sh.o_empty, o_phase, args.wait));
+                            ok = wait_v(nv) && (j || mbar_wait(&sh.o_empty, o_phase, args.wait)) && product(t, nv % V_STAGES, j > 1);
                             if (!ok) break;
-                            after();
-                            product(t, nv % V_STAGES, j > 1);
                             umma_commit(&sh.v_empty[nv % V_STAGES]);
                             if (j + 2 < nb) {
                                 if (!wait_k(nk)) { ok = false; break; }
@@ -583,11 +589,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             packed[i] = pack2<T>(x, y);
                         }
                         tmem_st32(s_addr + half * 32, packed);
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_full[t][half]);
                     }
+                } else {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane < 2) mbar_arrive(&sh.p_full[t][lane]);
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
             }
             float l;
             {
@@ -690,7 +700,7 @@ int launch_tc(TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUt
     XN_ENSURE_SMEM(kern, smem);
     a.p.parts = sm_count();
     if (int rc = launch_dependent(kern, dim3((unsigned)a.p.parts), dim3(TC_THREADS), smem, st, mq, mk, mv, a)) return rc;
-    return launch_paged_merge(FMT_OF<T>, HD, TC_ROWS, a.tile_tokens * a.p.group, 1, a.p, st);
+    return launch_paged_merge(FMT_OF<T>, HD, TC_ROWS, a.tile_tokens * a.p.group, a.p, st);
 }
 
 }  // namespace

@@ -47,12 +47,12 @@ __device__ __forceinline__ Sequence load_sequence(const PagedArgs &a, int b) {
 }
 
 // A row's result over a part of its keys: the sum of p v (head_dim floats), the maximum m of its scaled scores and the sum l of
-// p = 2^(score - m).  CTA c of `parts` writes the part that it did not begin into record 0 and the part that it does not end
-// into record 1, and leaves a note of the latter.
+// p = 2^(score - m).  CTA c of `parts` writes the part of the item that began before it into record 0 and the part of the one that it
+// begins and does not end into record 1, and leaves a note of both.
 struct PartNote {
-    unsigned long long begin, end, total;  // the item's units, and all units of the call; end == 0: no note
-    int q0, rows, tile_row, head;          // first query row of its sequence, rows of the sequence, first row of the item, kv head
-    int step;                              // units per key block: a CTA holds the blocks that begin in its share
+    int joined;                    // whether record 0 is written
+    int last;                      // record 1 is: the item goes on in the CTAs behind this one, up to this one (0: it is not)
+    int q0, rows, tile_row, head;  // the item's: first query row of its sequence, rows of the sequence, first row of the item, kv head
 };
 __host__ __device__ constexpr size_t part_record_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 __host__ __device__ constexpr size_t part_bytes(int parts, int rows, int hd) {
@@ -64,6 +64,17 @@ __host__ __device__ inline float *part_records(void *ws, int parts) {
 // Units are dealt out evenly, in order: share g of `shares` gets [share_begin(g), share_begin(g + 1)).
 __host__ __device__ __forceinline__ unsigned long long share_begin(unsigned long long total, unsigned g, unsigned shares) {
     return total / shares * g + total % shares * g / shares;
+}
+
+// The share that unit x of `total` falls into.
+__device__ __forceinline__ unsigned share_of(unsigned long long x, unsigned long long total, unsigned shares) {
+    unsigned lo = 0, hi = shares - 1;
+    while (lo < hi) {
+        const unsigned mid = (lo + hi + 1) >> 1;
+        if (share_begin(total, mid, shares) <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
 }
 
 template <typename T> constexpr xn_dtype FMT_OF = std::is_same<T, __half>::value ? XN_F16 : XN_BF16;
@@ -85,8 +96,8 @@ __device__ __forceinline__ float exp2_fast(float x) {  // relative error about 2
 // attention_paged_stream.cu: up to 16 rows of a key head at a time, any page size
 int launch_paged_stream(xn_dtype dt, int head_dim, int rows, PagedArgs &a, cudaStream_t st);
 size_t paged_stream_workspace(int head_dim);
-// Records of `rows` rows, of which the first `used` of every 128 are rows of the item; a CTA of `a.parts` has `shares` shares.
-int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, int shares, const PagedArgs &a, cudaStream_t st);
+// Records of `rows` rows, of which the first `used` of every 128 are rows of the item.
+int launch_paged_merge(xn_dtype dt, int head_dim, int rows, int used, const PagedArgs &a, cudaStream_t st);
 // attention_paged_tc.cu: 256 rows of a key head at a time on the tensor-memory MMAs; pages of a multiple of 8 rows
 bool paged_tc_fits(const PagedArgs &a);
 size_t paged_tc_workspace(int head_dim);
