@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         at = block_scan(mine, sum);
         total += sum;
     }
-    const unsigned shares = gridDim.x * WARPS, share = blockIdx.x * WARPS + warp;
+    const Shares shares(total, gridDim.x * WARPS);
+    const unsigned share = blockIdx.x * WARPS + warp;
     unsigned long long seen = 0;
     for (int r = 0; r < rounds; ++r) {
         const int b = r * WARPS * 32 + (int)threadIdx.x;
@@ -153,18 +154,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
             mine = b < a.batch ? sequence_units<TR>(a, b).total(a) : 0;
             at = block_scan(mine, sum);
         }
-        for (int w = 0; w < WARPS; ++w) {
-            const unsigned long long p = share_begin(total, blockIdx.x * WARPS + w, shares);
-            if (p >= seen + at && p < seen + at + mine) {
-                start_b[w] = b;
-                start_base[w] = seen + at;
+        if (mine)
+            for (int w = 0; w < WARPS; ++w) {
+                const unsigned long long p = shares.begin(blockIdx.x * WARPS + w);
+                if (p >= seen + at && p < seen + at + mine) {
+                    start_b[w] = b;
+                    start_base[w] = seen + at;
+                }
             }
-        }
         seen += sum;
     }
     if (lane == 0) heads[2 * warp].end = heads[2 * warp + 1].end = 0;
     __syncthreads();
-    const unsigned long long first = share_begin(total, share, shares), last = share_begin(total, share + 1, shares);
+    const unsigned long long first = shares.begin(share), last = shares.begin(share + 1);
 
     unsigned char *ring = smem + warp * STAGES * STAGE;
     auto store_part = [&](int which, const Cursor &c, const float (&o)[HD / 16][NT][4], const float (&m)[NT][2], const float (&l)[NT][2]) {
@@ -191,11 +193,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         pc.b = start_b[warp];
         pc.u = sequence_units<TR>(a, pc.b);
         {
-            const unsigned long long rem = first - start_base[warp];
-            const unsigned item = (unsigned)(rem / (unsigned)pc.u.U);
-            pc.unit = (int)(rem % (unsigned)pc.u.U);
-            pc.head = (int)(item / (unsigned)pc.u.tiles);
-            pc.tile = (int)(item % (unsigned)pc.u.tiles);
+            unsigned long long item, unit;
+            divide(first - start_base[warp], (unsigned)pc.u.U, item, unit);
+            pc.unit = (int)unit;
+            pc.head = (int)((unsigned)item / (unsigned)pc.u.tiles);
+            pc.tile = (int)((unsigned)item % (unsigned)pc.u.tiles);
         }
         Cursor cc = pc;  // what is computed next
         int page = -1;   // the page of this lane's key in the unit at pc: read one unit ahead
@@ -382,8 +384,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
     __syncthreads();
 
     // ---- parts of one item within the CTA are joined; what began before it or goes on behind it becomes a record ----
-    const unsigned long long cta_first = share_begin(total, blockIdx.x * WARPS, shares);
-    const unsigned long long cta_last = share_begin(total, (blockIdx.x + 1) * WARPS, shares);
+    const unsigned long long cta_first = shares.begin(blockIdx.x * WARPS), cta_last = shares.begin((blockIdx.x + 1) * WARPS);
     PartNote *note = static_cast<PartNote *>(a.ws) + blockIdx.x;
     float *out_rec = part_records(a.ws, gridDim.x) + (size_t)blockIdx.x * 2 * REC;
     PartNote said{};
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         }
         if (!whole && which == 0) said.joined = 1;
         if (!whole && which == 1 && threadIdx.x == 0)
-            said = PartNote{said.joined, (int)(share_of(h.end - 1, total, shares) / WARPS), h.q0, h.rows, h.tile_row, h.head};
+            said = PartNote{said.joined, (int)(shares.of(h.end - 1) / WARPS), h.q0, h.rows, h.tile_row, h.head};
         i = j;
     }
     if (threadIdx.x == 0) *note = said;

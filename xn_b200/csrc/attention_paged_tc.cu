@@ -28,7 +28,7 @@ constexpr int TC_THREADS = 128 + 256;      // TMA producer, MMA issuer, segment 
 constexpr int TC_WARPS = TC_THREADS / 32;
 constexpr int KEYS = 128;
 constexpr int HALF = KEYS * BKB;           // 128 rows of 64 elements: 16 KB
-constexpr int K_STAGES = 3, V_STAGES = 2;
+constexpr int K_STAGES = 2, V_STAGES = 2;
 constexpr int TC_ROWS = 256;               // rows of an item and of a record
 constexpr int SEGS = 4;                    // segments that the walker may be ahead
 
@@ -120,6 +120,7 @@ struct TcShared {
     uint64_t q_full, q_empty, k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty, red_full, red_empty, seg_full[SEGS], seg_empty[SEGS];
     u64 scan[TC_WARPS], start_base, start_sum;
+    TcSequence start_seq;  // the sequence that the CTA's share begins in
     Segment segs[SEGS];
     uint32_t tmem_slot;
     int start_b;
@@ -170,7 +171,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     unsigned char *sQ = smem;                     // two tiles
     unsigned char *sK = sQ + 2 * STAGE;
     unsigned char *sV = sK + K_STAGES * STAGE;
-    TcShared &sh = *reinterpret_cast<TcShared *>(sV + V_STAGES * STAGE);
+    unsigned char *sOut = sV + V_STAGES * STAGE;  // 4 KB for each softmax warp
+    TcShared &sh = *reinterpret_cast<TcShared *>(sOut + 8 * 4096);
     const int warp = warp_id(), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -207,8 +209,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     // ---- where this CTA's share begins ----
     // units of a sequence per key head; a sequence of many items is added up by its whole warp
+    TcSequence mine_seq{};
     auto sequence_sum = [&](int b) -> u64 {
-        TcSequence q{};
+        TcSequence &q = mine_seq;
+        q = TcSequence{};
         if (b < p.batch) q = tc_sequence(args, b);
         u64 sum = 0;
         if (q.supers <= 4)
@@ -255,7 +259,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         at = block_scan(mine * (unsigned)p.kv_heads, sum);
         total += sum;
     }
-    const u64 first = share_begin(total, blockIdx.x, gridDim.x), last = share_begin(total, blockIdx.x + 1, gridDim.x);
+    const Shares shares(total, gridDim.x);
+    const u64 first = shares.begin(blockIdx.x), last = shares.begin(blockIdx.x + 1);
     u64 seen = 0;
     for (int r = 0; r < rounds; ++r) {
         u64 sum = total;
@@ -266,6 +271,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const u64 begin = seen + at;
         if (first >= begin && first < begin + mine * (unsigned)p.kv_heads) {
             sh.start_b = r * TC_THREADS + (int)threadIdx.x;
+            sh.start_seq = mine_seq;
             sh.start_base = begin;
             sh.start_sum = mine;
         }
@@ -348,9 +354,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 walk.b = sh.start_b;
                 walk.first = first;
                 walk.last = last;
-                walk.q = tc_sequence(args, sh.start_b);
-                const u64 rem = first - sh.start_base, in_head = rem % sh.start_sum;
-                n_head = (int)(rem / sh.start_sum);
+                walk.q = sh.start_seq;
+                u64 head, in_head;
+                divide(first - sh.start_base, sh.start_sum, head, in_head);
+                n_head = (int)head;
                 u64 before = 0;
                 for (int i0 = 0; i0 < walk.q.supers; i0 += 32) {  // the item that the share begins in
                     const u64 c = i0 + lane < walk.q.supers ? tc_cost(args, walk.q.s.n, walk.q.s.off, i0 + lane) : 0;
@@ -374,7 +381,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const bool more = walk.next(args, g, &begin, &end);
                     if (more && g.record == 0) note.joined = 1;
                     if (more && g.record == 1)
-                        note = PartNote{note.joined, (int)share_of(end - 1, total, gridDim.x), g.row0 - g.tok0, g.n * p.group, g.tok0 * p.group, g.head};
+                        note = PartNote{note.joined, (int)shares.of(end - 1), g.row0 - g.tok0, g.n * p.group, g.tok0 * p.group, g.head};
                     if (!more) g.nb = 0;
                     const unsigned slot = n_seg % SEGS;
                     if (!mbar_wait(&sh.seg_empty[slot], ((n_seg / SEGS) & 1u) ^ 1u, args.wait)) break;
@@ -542,8 +549,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (real && (key0 + KEYS - 1 > horizon || key0 < low)) {
 #pragma unroll
-                        for (int i = 0; i < KEYS; ++i)
-                            if (key0 + i > horizon || key0 + i < low) v[i >> 5][i & 31] = 0xff800000u;
+                        for (int c = 0; c < 4; ++c) {
+                            // bits [from, to) of the chunk's columns are seen
+                            const int from = min(max(low - key0 - 32 * c, 0), 32), to = min(max(horizon + 1 - key0 - 32 * c, 0), 32);
+                            const uint32_t seen = (uint32_t)((1ull << to) - 1) & ~(uint32_t)((1ull << from) - 1);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (!(seen & (1u << i))) v[c][i] = 0xff800000u;
+                        }
                     }
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -630,46 +643,52 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const bool empty = l == 0.0f;
                 const float inv = empty ? 0.0f : 1.0f / l;
-                // columns of the row that this thread writes: all of its tile's accumulator, or half of both
+                // Columns of the row that this thread reads: all of its tile's accumulator, or half of both.  32 at a time go through shared
+                // memory, so that eight threads write 32 columns of one row together: a thread that wrote its own row would touch a line
+                // of its own with every store.
                 const int c0 = dual ? 0 : t * (HD / 2), ncols = dual ? HD : HD / 2;
                 const int record = g.record;
                 float *rec = part_records(p.ws, gridDim.x) + ((size_t)blockIdx.x * 2 + max(record, 0)) * part_record_floats(TC_ROWS, HD);
                 const int rec_row = dual ? t * 128 + r : r;
-                T *dst = static_cast<T *>(p.out) + (long long)(g.row0 - g.tok0 + tok) * p.out_token + (long long)(g.head * p.group + r_head) * p.out_head;
+                const long long own_row = !real ? -1
+                                          : record >= 0 ? (long long)rec_row * HD
+                                                        : (long long)(g.row0 - g.tok0 + tok) * p.out_token + (long long)(g.head * p.group + r_head) * p.out_head;
                 if (any_real) {
+                    const float scale0 = record >= 0 ? w0 : w0 * inv, scale1 = record >= 0 ? w1 : w1 * inv;
+                    float4 *mine = reinterpret_cast<float4 *>(sOut + (warp - 4) * 4096);
+                    long long rows[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xffffffffu, own_row, 4 * i + (lane >> 3));
 #pragma unroll 1
                     for (int c = c0; c < c0 + ncols; c += 32) {
-                        uint32_t x[32];
-                        float f[32];
+                        uint32_t x[32], y[32];
                         if (dual) {
                             tmem_ld32(o_addr + c, x);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(x[i]);
                         } else {
-                            uint32_t y[32];
                             tmem_ld32_nowait(lanes + 256 + c, x);
                             tmem_ld32_nowait(lanes + 256 + HD + c, y);
                             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                f[i] = (w0 == 0.0f ? 0.0f : __uint_as_float(x[i]) * w0) + (w1 == 0.0f ? 0.0f : __uint_as_float(y[i]) * w1);
                         }
-                        if (!real) continue;
-                        if (record < 0) {
+                        __syncwarp();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                uint4 o;
-                                o.x = pack2<T>(empty ? 0.0f : f[i] * inv, empty ? 0.0f : f[i + 1] * inv);
-                                o.y = pack2<T>(empty ? 0.0f : f[i + 2] * inv, empty ? 0.0f : f[i + 3] * inv);
-                                o.z = pack2<T>(empty ? 0.0f : f[i + 4] * inv, empty ? 0.0f : f[i + 5] * inv);
-                                o.w = pack2<T>(empty ? 0.0f : f[i + 6] * inv, empty ? 0.0f : f[i + 7] * inv);
-                                *reinterpret_cast<uint4 *>(dst + c + i) = o;
+                        for (int i = 0; i < 8; ++i) {
+                            float f[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                f[e] = scale0 == 0.0f || empty ? 0.0f : __uint_as_float(x[4 * i + e]) * scale0;
+                                if (!dual && scale1 != 0.0f && !empty) f[e] += __uint_as_float(y[4 * i + e]) * scale1;
                             }
-                        } else {
+                            mine[lane * 8 + (i ^ (lane & 7))] = make_float4(f[0], f[1], f[2], f[3]);
+                        }
+                        __syncwarp();
 #pragma unroll
-                            for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<float4 *>(rec + (size_t)rec_row * HD + c + i) =
-                                    empty ? make_float4(0, 0, 0, 0) : make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+                        for (int i = 0; i < 8; ++i) {
+                            const int row = 4 * i + (lane >> 3), piece = lane & 7;
+                            const float4 f = mine[row * 8 + (piece ^ (row & 7))];
+                            if (rows[i] < 0) continue;
+                            if (record >= 0) *reinterpret_cast<float4 *>(rec + rows[i] + c + piece * 4) = f;
+                            else
+                                *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + rows[i] + c + piece * 4) = make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
                         }
                     }
                 }
@@ -696,7 +715,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 template <typename T, int HD>
 int launch_tc(TcArgs &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
     auto kern = paged_tc_kernel<T, HD>;
-    const size_t smem = (size_t)(2 + K_STAGES + V_STAGES) * (HD / 64) * HALF + sizeof(TcShared);
+    const size_t smem = (size_t)(2 + K_STAGES + V_STAGES) * (HD / 64) * HALF + 8 * 4096 + sizeof(TcShared);
     XN_ENSURE_SMEM(kern, smem);
     a.p.parts = sm_count();
     if (int rc = launch_dependent(kern, dim3((unsigned)a.p.parts), dim3(TC_THREADS), smem, st, mq, mk, mv, a)) return rc;

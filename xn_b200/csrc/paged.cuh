@@ -61,20 +61,40 @@ __host__ __device__ constexpr size_t part_bytes(int parts, int rows, int hd) {
 __host__ __device__ inline float *part_records(void *ws, int parts) {
     return reinterpret_cast<float *>(static_cast<char *>(ws) + ((size_t)parts * sizeof(PartNote) + 255) / 256 * 256);
 }
-// Units are dealt out evenly, in order: share g of `shares` gets [share_begin(g), share_begin(g + 1)).
-__host__ __device__ __forceinline__ unsigned long long share_begin(unsigned long long total, unsigned g, unsigned shares) {
-    return total / shares * g + total % shares * g / shares;
-}
-
-// The share that unit x of `total` falls into.
-__device__ __forceinline__ unsigned share_of(unsigned long long x, unsigned long long total, unsigned shares) {
-    unsigned lo = 0, hi = shares - 1;
-    while (lo < hi) {
-        const unsigned mid = (lo + hi + 1) >> 1;
-        if (share_begin(total, mid, shares) <= x) lo = mid;
-        else hi = mid - 1;
+// Units are dealt out evenly, in order: share g of `count` gets [begin(g), begin(g + 1)).  The 64-bit divisions that are not needed are
+// left out: they would take longer than the rest of a short call's way to its first load.
+struct Shares {
+    unsigned long long total, each;
+    unsigned rest, count;
+    __device__ __forceinline__ Shares(unsigned long long units, unsigned shares) : total(units), count(shares) {
+        if (units >> 32) {
+            each = units / shares;
+            rest = (unsigned)(units % shares);
+        } else {
+            each = (unsigned)units / shares;
+            rest = (unsigned)units % shares;
+        }
     }
-    return lo;
+    __device__ __forceinline__ unsigned long long begin(unsigned g) const { return each * g + rest * g / count; }  // below 2^16 shares
+    // the share that a unit falls into
+    __device__ __forceinline__ unsigned of(unsigned long long unit) const {
+        unsigned lo = 0, hi = count - 1;
+        while (lo < hi) {
+            const unsigned mid = (lo + hi + 1) >> 1;
+            if (begin(mid) <= unit) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+};
+__device__ __forceinline__ void divide(unsigned long long x, unsigned long long by, unsigned long long &quotient, unsigned long long &rest) {
+    if ((x | by) >> 32) {
+        quotient = x / by;
+        rest = x % by;
+    } else {
+        quotient = (unsigned)x / (unsigned)by;
+        rest = (unsigned)x % (unsigned)by;
+    }
 }
 
 template <typename T> constexpr xn_dtype FMT_OF = std::is_same<T, __half>::value ? XN_F16 : XN_BF16;
