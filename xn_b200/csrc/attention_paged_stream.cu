@@ -455,45 +455,47 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
     const PartNote n = notes[blockIdx.x];
     if (n.last == 0) return;
     const int in_block = threadIdx.x / (LANES * SLICES), slice = threadIdx.x / LANES % SLICES, lane = threadIdx.x % LANES;
-    const int row = blockIdx.y * ROWS + in_block;
-    const int item_row = (row >> 7) * used + (row & 127);
-    const bool real = row < rec_rows && (row & 127) < used && n.tile_row + item_row < n.rows;
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    auto join = [&](float rm, float rl, const float4 &ro) {
-        const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
-        const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
-        l = l * w0 + rl * w1;
-        o.x = o.x * w0 + ro.x * w1;
-        o.y = o.y * w0 + ro.y * w1;
-        o.z = o.z * w0 + ro.z * w1;
-        o.w = o.w * w0 + ro.w * w1;
-        m = mn;
-    };
-    if (real)
-        for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
-            if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
-            const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-            join(rec[rec_rows * HD + row], rec[rec_rows * HD + rec_rows + row], reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane]);
+    for (int row0 = blockIdx.y * ROWS; row0 < rec_rows; row0 += gridDim.y * ROWS) {
+        const int row = row0 + in_block;
+        const int item_row = (row >> 7) * used + (row & 127);
+        const bool real = (row & 127) < used && n.tile_row + item_row < n.rows;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0, 0, 0, 0);
+        auto join = [&](float rm, float rl, const float4 &ro) {
+            const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
+            const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
+            l = l * w0 + rl * w1;
+            o.x = o.x * w0 + ro.x * w1;
+            o.y = o.y * w0 + ro.y * w1;
+            o.z = o.z * w0 + ro.z * w1;
+            o.w = o.w * w0 + ro.w * w1;
+            m = mn;
+        };
+        if (real)
+            for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
+                if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
+                const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
+                join(rec[rec_rows * HD + row], rec[rec_rows * HD + rec_rows + row], reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane]);
+            }
+        if (SLICES > 1) {  // one row a block
+            so[in_block][slice][lane] = o;
+            if (lane == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
+            __syncthreads();
+            if (slice) return;
+            for (int s = 1; s < SLICES; ++s) join(sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
         }
-    if (SLICES > 1) {
-        so[in_block][slice][lane] = o;
-        if (lane == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
-        __syncthreads();
-        if (slice) return;
-        for (int s = 1; s < SLICES; ++s) join(sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
+        if (!real) continue;
+        const unsigned r = (unsigned)(n.tile_row + item_row);
+        T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
+                 (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint2 w;
+        w.x = pack2<T>(o.x * inv, o.y * inv);
+        w.y = pack2<T>(o.z * inv, o.w * inv);
+        reinterpret_cast<uint2 *>(dst)[lane] = w;
     }
-    if (!real) return;
-    const unsigned r = (unsigned)(n.tile_row + item_row);
-    T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
-             (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint2 w;
-    w.x = pack2<T>(o.x * inv, o.y * inv);
-    w.y = pack2<T>(o.z * inv, o.w * inv);
-    reinterpret_cast<uint2 *>(dst)[lane] = w;
 }
 
 template <int HD, int NT> struct StreamShape {
@@ -519,7 +521,7 @@ template <typename T, int HD> int launch_merge(int rows, int used, const PagedAr
     constexpr int ROWS = MERGE_NT * 4 / HD;
     if (rows <= 16)
         return launch_dependent(paged_merge_kernel<T, HD, ROWS>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
-    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS - 1) / ROWS)), dim3(MERGE_NT), 0, st,
+    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, 8), dim3(MERGE_NT), 0, st,
                             a, rows, used);
 }
 }  // namespace
