@@ -443,9 +443,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
 }
 
 // Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
-// of the CTAs behind it.  A thread holds four columns of a row; SLICES groups of threads share a row's records.
+// of the CTAs behind it.  A thread holds four columns of AT rows at once; SLICES groups of threads share a row's records.
 constexpr int MERGE_NT = 256;
-template <typename T, int HD, int SLICES>
+template <typename T, int HD, int SLICES, int AT>
 __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
     constexpr int LANES = HD / 4, ROWS = MERGE_NT / LANES / SLICES;
     __shared__ float sm[ROWS][SLICES], sl[ROWS][SLICES];
@@ -457,43 +457,62 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
     const int in_block = threadIdx.x / (LANES * SLICES), slice = threadIdx.x / LANES % SLICES, lane = threadIdx.x % LANES;
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
-    for (int row0 = blockIdx.y * ROWS; row0 < rec_rows; row0 += gridDim.y * ROWS) {
-        const int row = row0 + in_block;
-        const int item_row = (row >> 7) * used + (row & 127);
-        const bool real = (row & 127) < used && n.tile_row + item_row < n.rows;
-        float m = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0, 0, 0, 0);
-        auto join = [&](float rm, float rl, const float4 &ro) {
-            const float mn = fmaxf(m, rm), ref = mn == -INFINITY ? 0.0f : mn;
-            const float w0 = exp2_fast(m - ref), w1 = exp2_fast(rm - ref);
-            l = l * w0 + rl * w1;
-            o.x = o.x * w0 + ro.x * w1;
-            o.y = o.y * w0 + ro.y * w1;
-            o.z = o.z * w0 + ro.z * w1;
-            o.w = o.w * w0 + ro.w * w1;
-            m = mn;
-        };
-        if (real)
-            for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
-                if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
-                const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-                join(rec[rec_rows * HD + row], rec[rec_rows * HD + rec_rows + row], reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane]);
-            }
-        if (SLICES > 1) {  // one row a block
-            so[in_block][slice][lane] = o;
-            if (lane == 0) { sm[in_block][slice] = m; sl[in_block][slice] = l; }
-            __syncthreads();
-            if (slice) return;
-            for (int s = 1; s < SLICES; ++s) join(sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
+    float m[AT], l[AT];
+    float4 o[AT];
+    int rows[AT], item_rows[AT];
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+        const int row = (blockIdx.y * AT + i) * ROWS + in_block, item_row = n.tile_row + (row >> 7) * used + (row & 127);
+        const bool real = row < rec_rows && (row & 127) < used && item_row < n.rows;
+        rows[i] = real ? row : -1;
+        item_rows[i] = item_row;
+        m[i] = -INFINITY;
+        l[i] = 0.0f;
+        o[i] = make_float4(0, 0, 0, 0);
+    }
+    auto join = [&](int i, float rm, float rl, const float4 &ro) {
+        const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
+        const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
+        l[i] = l[i] * w0 + rl * w1;
+        o[i].x = o[i].x * w0 + ro.x * w1;
+        o[i].y = o[i].y * w0 + ro.y * w1;
+        o[i].z = o[i].z * w0 + ro.z * w1;
+        o[i].w = o[i].w * w0 + ro.w * w1;
+        m[i] = mn;
+    };
+    for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
+        if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
+        const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
+        float rm[AT], rl[AT];
+        float4 ro[AT];
+#pragma unroll
+        for (int i = 0; i < AT; ++i) {
+            const int row = max(rows[i], 0);  // a row that nobody has is not written
+            rm[i] = rows[i] >= 0 ? rec[rec_rows * HD + row] : -INFINITY;
+            rl[i] = rows[i] >= 0 ? rec[rec_rows * HD + rec_rows + row] : 0.0f;
+            ro[i] = rows[i] >= 0 ? reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane] : make_float4(0, 0, 0, 0);
         }
-        if (!real) continue;
-        const unsigned r = (unsigned)(n.tile_row + item_row);
+#pragma unroll
+        for (int i = 0; i < AT; ++i) join(i, rm[i], rl[i], ro[i]);
+    }
+    if (SLICES > 1) {
+        static_assert(SLICES == 1 || AT == 1, "a row's slices are joined for one row at a time");
+        so[in_block][slice][lane] = o[0];
+        if (lane == 0) { sm[in_block][slice] = m[0]; sl[in_block][slice] = l[0]; }
+        __syncthreads();
+        if (slice) return;
+        for (int s = 1; s < SLICES; ++s) join(0, sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
+    }
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+        if (rows[i] < 0) continue;
+        const unsigned r = (unsigned)item_rows[i];
         T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
                  (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
         uint2 w;
-        w.x = pack2<T>(o.x * inv, o.y * inv);
-        w.y = pack2<T>(o.z * inv, o.w * inv);
+        w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
+        w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
         reinterpret_cast<uint2 *>(dst)[lane] = w;
     }
 }
@@ -518,11 +537,11 @@ template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream
 namespace {
 // Few rows may have a record from every CTA: all threads of a block share one row's.  Many rows have a few each.
 template <typename T, int HD> int launch_merge(int rows, int used, const PagedArgs &a, cudaStream_t st) {
-    constexpr int ROWS = MERGE_NT * 4 / HD;
+    constexpr int ROWS = MERGE_NT * 4 / HD, AT = 4;
     if (rows <= 16)
-        return launch_dependent(paged_merge_kernel<T, HD, ROWS>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
-    return launch_dependent(paged_merge_kernel<T, HD, 1>, dim3((unsigned)a.parts, 8), dim3(MERGE_NT), 0, st,
-                            a, rows, used);
+        return launch_dependent(paged_merge_kernel<T, HD, ROWS, 1>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
+    return launch_dependent(paged_merge_kernel<T, HD, 1, AT>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS * AT - 1) / (ROWS * AT))), dim3(MERGE_NT),
+                            0, st, a, rows, used);
 }
 }  // namespace
 

@@ -24,11 +24,12 @@ namespace xn {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int TC_THREADS = 128 + 256;      // TMA producer, MMA issuer, segment walker, an idle warp; two softmax warpgroups
+constexpr int TC_THREADS = 128 + 256;      // two TMA producers, MMA issuer, segment walker; two softmax warpgroups
 constexpr int KEYS = 128;
 constexpr int HALF = KEYS * BKB;           // 128 rows of 64 elements: 16 KB
 constexpr int K_STAGES = 2, V_STAGES = 2;
 constexpr int TC_ROWS = 256;               // rows of an item and of a record
+constexpr u64 SNAP = 4 * 2 * KEYS;          // units, see tc_weight
 constexpr int SEGS = 4;                    // segments that the walker may be ahead
 
 struct TcArgs {
@@ -115,9 +116,15 @@ struct Walk {
             const int nkb = it.kb1 - it.kb0, dual = it.dual;
             const u64 units = tc_weight(a, q, index);
             *end = pos + units;
-            // the blocks that begin in this share, if they lie evenly in the item's units
-            const int from = first > pos ? (int)(((first - pos) * (unsigned)nkb + units - 1) / units) : 0;
-            const int to = last < *end ? (int)(((last - pos) * (unsigned)nkb + units - 1) / units) : nkb;
+            // The blocks that begin in this share, if they lie evenly in the item's units.  A share's end that is near one of the item's is
+            // moved there: a part of an item costs a record of its rows, as much as two blocks.
+            auto cut = [&](u64 at) {
+                if (at >= *end) return nkb;
+                if (at <= pos || at - pos < SNAP) return 0;
+                if (*end - at < SNAP) return nkb;
+                return (int)(((at - pos) * (unsigned)nkb + units - 1) / units);
+            };
+            const int from = cut(first), to = cut(last);
             g = Segment{to - from, it.kb0 + from, b, head, q.s.q0 + it.tok0, it.tok0, q.s.n, q.s.ctx, q.s.off, it.lo, dual,
                         from == 0 && to == nkb ? -1 : (from > 0 ? 0 : 1)};
             pos = *end;
@@ -200,7 +207,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         mbar_init(&sh.o_empty, 8);
         mbar_init(&sh.red_full, 8);
         mbar_init(&sh.red_empty, 8);
-        for (int i = 0; i < SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_empty[i], 10); }
+        for (int i = 0; i < SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_empty[i], 11); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -222,13 +229,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     // that the launch has (384 x 168).
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0) {
-            // ---- producer: lane i looks after piece i of a key block ----
+        if (warp == 0 || warp == 3) {
+            // ---- producers, one of Q and K, one of V: lane i looks after piece i of a key block ----
             asm volatile("griddepcontrol.wait;" ::: "memory");
+            const bool keys = warp == 0;
+            const CUtensorMap *map = keys ? &map_k : &map_v;
             bool ok = true;
             unsigned n_block = 0;
             const int pieces = KEYS / args.box;
             const unsigned tile_bytes = (unsigned)(args.tile_tokens * p.group * BKB * H);
+            static_assert(K_STAGES == V_STAGES, "one stage count for both rings");
             for (unsigned n_seg = 0; ok; ++n_seg) {
                 const unsigned slot = n_seg % SEGS;
                 if (!wait_all(&sh.seg_full[slot], (n_seg / SEGS) & 1u)) break;
@@ -245,7 +255,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         page = p.table[(long long)g.b * p.table_stride + at_page];
                     }
                 };
-                auto load_q = [&]() {
+                fetch(g.kb0);
+                if (keys) {  // while the first page's index is on its way
+                    ok = wait_all(&sh.q_empty, (n_seg & 1u) ^ 1u);
+                    if (!ok) break;
                     if (elect_one()) {
                         mbar_expect_tx(&sh.q_full, tile_bytes << g.dual);
                         for (int t = 0; t <= g.dual; ++t)
@@ -253,36 +266,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             for (int h = 0; h < H; ++h)
                                 tma_load_3d(sQ + t * STAGE + h * HALF, &map_q, h * 64, g.head * p.group, g.row0 + t * args.tile_tokens, &sh.q_full);
                     }
-                };
-                fetch(g.kb0);
+                }
                 for (int kb = g.kb0; kb < g.kb0 + g.nb; ++kb, ++n_block) {
                     const int used = min(pieces, max(0, (g.ctx - kb * KEYS + args.box - 1) / args.box));
                     const int now_page = page, now_row = row;
                     fetch(kb + 1);
-                    auto load = [&](unsigned char *dst, const CUtensorMap *map, uint64_t *bar) {
-                        if (elect_one()) mbar_expect_tx(bar, (unsigned)(used * args.box * BKB * H));
-                        for (int i = 0; i < used; ++i) {
-                            const int pg = __shfl_sync(0xffffffffu, now_page, i), rw = __shfl_sync(0xffffffffu, now_row, i);
-                            if (elect_one()) {
-    #pragma unroll
-                                for (int h = 0; h < H; ++h)
-                                    tma_load_4d(dst + h * HALF + i * args.box * BKB, map, h * 64, rw, g.head, pg, bar);
-                            }
+                    const unsigned stage = n_block % K_STAGES, parity = ((n_block / K_STAGES) & 1u) ^ 1u;
+                    uint64_t *full = keys ? &sh.k_full[stage] : &sh.v_full[stage];
+                    ok = wait_all(keys ? &sh.k_empty[stage] : &sh.v_empty[stage], parity);
+                    if (!ok) break;
+                    unsigned char *dst = (keys ? sK : sV) + stage * STAGE;
+                    if (elect_one()) mbar_expect_tx(full, (unsigned)(used * args.box * BKB * H));
+                    for (int i = 0; i < used; ++i) {
+                        const int pg = __shfl_sync(0xffffffffu, now_page, i), rw = __shfl_sync(0xffffffffu, now_row, i);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int h = 0; h < H; ++h) tma_load_4d(dst + h * HALF + i * args.box * BKB, map, h * 64, rw, g.head, pg, full);
                         }
-                    };
-                    const unsigned ks = n_block % K_STAGES, vs = n_block % V_STAGES;
-                    if (kb == g.kb0 && n_seg == 0) load_q();  // nothing to wait for: ahead of the first page's index
-                    ok = wait_all(&sh.k_empty[ks], ((n_block / K_STAGES) & 1u) ^ 1u);
-                    if (!ok) break;
-                    load(sK + ks * STAGE, &map_k, &sh.k_full[ks]);
-                    if (kb == g.kb0 && n_seg) {
-                        ok = wait_all(&sh.q_empty, (n_seg & 1u) ^ 1u);
-                        if (!ok) break;
-                        load_q();
                     }
-                    ok = wait_all(&sh.v_empty[vs], ((n_block / V_STAGES) & 1u) ^ 1u);
-                    if (!ok) break;
-                    load(sV + vs * STAGE, &map_v, &sh.v_full[vs]);
                 }
                 if (lane == 0) mbar_arrive(&sh.seg_empty[slot]);
             }
