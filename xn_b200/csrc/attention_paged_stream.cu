@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         total += sum;
     }
     const Shares shares(total, gridDim.x * WARPS);
-    const unsigned share = blockIdx.x * WARPS + warp;
+    const unsigned long long bound = shares.begin(blockIdx.x * WARPS + min(lane, WARPS));  // lane w: where warp w's share begins
     unsigned long long seen = 0;
     for (int r = 0; r < rounds; ++r) {
         const int b = r * WARPS * 32 + (int)threadIdx.x;
@@ -154,19 +154,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
             mine = b < a.batch ? sequence_units<TR>(a, b).total(a) : 0;
             at = block_scan(mine, sum);
         }
-        if (mine)
-            for (int w = 0; w < WARPS; ++w) {
-                const unsigned long long p = shares.begin(blockIdx.x * WARPS + w);
-                if (p >= seen + at && p < seen + at + mine) {
-                    start_b[w] = b;
-                    start_base[w] = seen + at;
-                }
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const unsigned long long p = __shfl_sync(0xffffffffu, bound, w);
+            if (p >= seen + at && p < seen + at + mine) {
+                start_b[w] = b;
+                start_base[w] = seen + at;
             }
+        }
         seen += sum;
     }
     if (lane == 0) heads[2 * warp].end = heads[2 * warp + 1].end = 0;
     __syncthreads();
-    const unsigned long long first = shares.begin(share), last = shares.begin(share + 1);
+    const unsigned long long first = __shfl_sync(0xffffffffu, bound, warp), last = __shfl_sync(0xffffffffu, bound, warp + 1);
 
     unsigned char *ring = smem + warp * STAGES * STAGE;
     auto store_part = [&](int which, const Cursor &c, const float (&o)[HD / 16][NT][4], const float (&m)[NT][2], const float (&l)[NT][2]) {
@@ -203,14 +203,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         int page = -1;   // the page of this lane's key in the unit at pc: read one unit ahead
         auto key_of = [&](const Cursor &c) { return c.u.base + c.unit * UNIT + (lane & 15); };
         auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : (int)((unsigned)key / (unsigned)a.page_size); };
-        auto fetch_page = [&]() {
-            page = -1;
-            if (pc.pos < last) {
-                const int key = key_of(pc);
-                if (key >= pc.u.lo && key < pc.u.s.ctx) page = a.table[(long long)pc.b * a.table_stride + page_of(key)];
-            }
+        auto fetch_page = [&](const Cursor &c) {
+            const int key = key_of(c);
+            return c.pos < last && key >= c.u.lo && key < c.u.s.ctx ? a.table[(long long)c.b * a.table_stride + page_of(key)] : -1;
         };
-        auto issue = [&](int slot) {
+        auto issue = [&](int slot, int page) {
             if (pc.pos < last) {
                 const int key = key_of(pc);
                 const bool there = page >= 0 && page < a.num_pages;
@@ -230,13 +227,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                     cp_async16(vdst + d, static_cast<const T *>(a.v) + e, valid);
                 }
                 advance<TR>(a, pc);
-                fetch_page();
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        fetch_page();
+        {
+            int pages[STAGES];
+            Cursor c = pc;
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) issue(s);
+            for (int s = 0; s < STAGES; ++s) {
+                pages[s] = fetch_page(c);
+                if (c.pos < last) advance<TR>(a, c);
+            }
+#pragma unroll
+            for (int s = 0; s < STAGES - 1; ++s) issue(s, pages[s]);
+            page = pages[STAGES - 1];
+        }
 
         unsigned qf[HD / 16][NT][2];
         float o[HD / 16][NT][4], m[NT][2], l[NT][2];
@@ -277,7 +282,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
             }
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
             __syncwarp();
-            issue(slot == 0 ? STAGES - 1 : slot - 1);  // the slot of the unit before this one
+            issue(slot == 0 ? STAGES - 1 : slot - 1, page);  // the slot of the unit before this one
+            page = fetch_page(pc);
 
             const unsigned kt = smem_addr(ring + slot * STAGE), vt = kt + TILE;
             float s[NT][4];
@@ -384,39 +390,38 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
     __syncthreads();
 
     // ---- parts of one item within the CTA are joined; what began before it or goes on behind it becomes a record ----
-    const unsigned long long cta_first = shares.begin(blockIdx.x * WARPS), cta_last = shares.begin((blockIdx.x + 1) * WARPS);
-    PartNote *note = static_cast<PartNote *>(a.ws) + blockIdx.x;
+    const unsigned long long cta_first = __shfl_sync(0xffffffffu, bound, 0), cta_last = __shfl_sync(0xffffffffu, bound, WARPS);
     float *out_rec = part_records(a.ws, gridDim.x) + (size_t)blockIdx.x * 2 * REC;
     PartNote said{};
     auto rec_at = [&](int i) { return (i & 1) ? reinterpret_cast<const float *>(smem + (i >> 1) * STAGES * STAGE) : recs + (i >> 1) * REC; };
-    for (int i = 0; i < 2 * WARPS;) {
-        if (heads[i].end == 0) { ++i; continue; }
+    // lane i looks after record i of the 2 * WARPS: those of one item follow one another
+    const PartHead own = heads[min(lane, 2 * WARPS - 1)];
+    const unsigned there = __ballot_sync(0xffffffffu, lane < 2 * WARPS && own.end != 0);
+    const unsigned before = there & ((1u << lane) - 1);
+    const unsigned long long begin_before = __shfl_sync(0xffffffffu, own.begin, before ? 31 - __clz(before) : 0);
+    const unsigned leads = __ballot_sync(0xffffffffu, (there >> lane & 1) && (!before || begin_before != own.begin));
+    for (unsigned todo = leads; todo; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1, j = todo & (todo - 1) ? __ffs(todo & (todo - 1)) - 1 : 32;
+        const unsigned members = there & (j < 32 ? (1u << j) - 1 : ~0u) & ~((1u << i) - 1);
         const PartHead h = heads[i];
-        int j = i + 1;  // records [i, j) are of this item
-        for (int k = i + 1; k < 2 * WARPS; ++k)
-            if (heads[k].end != 0) {
-                if (heads[k].begin != h.begin) break;
-                j = k + 1;
-            }
         const bool whole = h.begin >= cta_first && h.end <= cta_last;
         const int which = h.begin < cta_first ? 0 : 1;
         const int rows = min(h.rows - h.tile_row, TR);
         for (int row = warp; row < rows; row += WARPS) {
-            float mm = -INFINITY;
-            for (int k = i; k < j; ++k)
-                if (heads[k].end) mm = fmaxf(mm, rec_at(k)[TR * HD + row]);
-            const float ref = mm == -INFINITY ? 0.0f : mm;
-            float ll = 0.0f, acc[HD / 32];
+            const bool member = members >> lane & 1;
+            const float *mine_rec = rec_at(member ? lane : i);
+            const float m = member ? mine_rec[TR * HD + row] : -INFINITY, l = member ? mine_rec[TR * HD + TR + row] : 0.0f;
+            const float mm = warp_max(m), w = mm == -INFINITY ? 0.0f : exp2_fast(m - mm), ll = warp_sum(w * l);
+            float acc[HD / 32];
 #pragma unroll
             for (int e = 0; e < HD / 32; ++e) acc[e] = 0.0f;
-            for (int k = i; k < j; ++k)
-                if (heads[k].end) {
-                    const float *rec = rec_at(k);
-                    const float w = exp2_fast(rec[TR * HD + row] - ref);
-                    ll += w * rec[TR * HD + TR + row];
+            for (unsigned k = members; k; k &= k - 1) {
+                const int at = __ffs(k) - 1;
+                const float wk = __shfl_sync(0xffffffffu, w, at);
+                const float *rec = rec_at(at) + row * HD + lane;
 #pragma unroll
-                    for (int e = 0; e < HD / 32; ++e) acc[e] += w * rec[row * HD + e * 32 + lane];
-                }
+                for (int e = 0; e < HD / 32; ++e) acc[e] += wk * rec[e * 32];
+            }
             if (whole) {
                 const unsigned r = (unsigned)(h.tile_row + row);
                 const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -437,9 +442,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         if (!whole && which == 0) said.joined = 1;
         if (!whole && which == 1 && threadIdx.x == 0)
             said = PartNote{said.joined, (int)(shares.of(h.end - 1) / WARPS), h.q0, h.rows, h.tile_row, h.head};
-        i = j;
     }
-    if (threadIdx.x == 0) *note = said;
+    if (threadIdx.x == 0) static_cast<PartNote *>(a.ws)[blockIdx.x] = said;
 }
 
 // Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0

@@ -11,7 +11,7 @@
 // know beforehand, and one thread's pairs keep their sine and cosine for all the heads that the thread turns.
 //
 // Bound: memory.  A thread moves a chunk of 2 x 16 bytes per head (16-bit elements: 8 pairs, f32: 4) where the sizes and the
-// alignment allow it, single pairs otherwise.
+// alignment allow it, single pairs otherwise; several heads share its sines and cosines.
 #include "common.cuh"
 
 namespace xn {
@@ -79,8 +79,9 @@ __global__ void __launch_bounds__(ROPE_NT) rope_kernel(const RopeArgs a) {
         const double pos = (double)a.positions[token];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const double t = pos * (a.freqs[chunk * V + j] * 0.15915494309189535);  // 1 / (2 pi)
-            sincospif((float)(2.0 * (t - rint(t))), &sn[j], &cs[j]);
+            // half turns, less the nearest even number of them: a sum with 1.5 * 2^53 is rounded to one
+            const double t = pos * (a.freqs[chunk * V + j] * 0.3183098861837907), k = t + 13510798882111488.0;
+            sincospif((float)(t - (k - 13510798882111488.0)), &sn[j], &cs[j]);
         }
     }
     // the two runs of the chunk within its head, with and without rotation
@@ -101,34 +102,53 @@ __global__ void __launch_bounds__(ROPE_NT) rope_kernel(const RopeArgs a) {
             slot += (long long)row * a.part[1].dst_token;
         }
     }
+    auto turn = [&](Chunk<T, V> &x0, Chunk<T, V> &x1) {
+        T u[2 * V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) { u[j] = x0.v[j]; u[V + j] = x1.v[j]; }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int ia = INTER ? 2 * j : j, ib = INTER ? 2 * j + 1 : V + j;
+            const float xa = to_f32(u[ia]), xb = to_f32(u[ib]);
+            u[ia] = from_f32<T>(xa * cs[j] - xb * sn[j]);
+            u[ib] = from_f32<T>(xa * sn[j] + xb * cs[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) { x0.v[j] = u[j]; x1.v[j] = u[V + j]; }
+    };
     int head = group;
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
         const RopePart &part = a.part[p];
-        for (; head < part.heads; head += a.head_groups) {
-            if (part.paged && !stored) continue;
-            const T *src = static_cast<const T *>(part.src) + (long long)token * part.src_token + (long long)head * part.src_head;
-            T *dst = static_cast<T *>(part.dst) + (part.paged ? slot : (long long)token * part.dst_token) + (long long)head * part.dst_head;
-            const int e0 = part.rotate ? turn0 : plain0, e1 = part.rotate ? turn1 : plain1;
-            Chunk<T, V> x0 = load_chunk<T, V>(src + e0), x1 = load_chunk<T, V>(src + e1);
-            if (part.rotate && turned) {
-                T u[2 * V];
+        const bool turns = part.rotate && turned;
+        const int e0 = part.rotate ? turn0 : plain0, e1 = part.rotate ? turn1 : plain1;
+        const T *src = static_cast<const T *>(part.src) + (long long)token * part.src_token;
+        T *dst = static_cast<T *>(part.dst) + (part.paged ? slot : (long long)token * part.dst_token);
+        if (part.paged && !stored) break;  // nor is the part behind
+        const int first = head;
+        constexpr int AT = 2;  // heads whose loads are in flight together
+        for (; head < part.heads; head += AT * a.head_groups) {
+            Chunk<T, V> x0[AT], x1[AT];
 #pragma unroll
-                for (int j = 0; j < V; ++j) { u[j] = x0.v[j]; u[V + j] = x1.v[j]; }
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int ia = INTER ? 2 * j : j, ib = INTER ? 2 * j + 1 : V + j;
-                    const float xa = to_f32(u[ia]), xb = to_f32(u[ib]);
-                    u[ia] = from_f32<T>(xa * cs[j] - xb * sn[j]);
-                    u[ib] = from_f32<T>(xa * sn[j] + xb * cs[j]);
+            for (int i = 0; i < AT; ++i) {
+                const int h = head + i * a.head_groups;
+                if (h < part.heads) {
+                    x0[i] = load_chunk<T, V>(src + (long long)h * part.src_head + e0);
+                    x1[i] = load_chunk<T, V>(src + (long long)h * part.src_head + e1);
                 }
-#pragma unroll
-                for (int j = 0; j < V; ++j) { x0.v[j] = u[j]; x1.v[j] = u[V + j]; }
             }
-            store_chunk<T, V>(dst + e0, x0);
-            store_chunk<T, V>(dst + e1, x1);
+#pragma unroll
+            for (int i = 0; i < AT; ++i) {
+                const int h = head + i * a.head_groups;
+                if (h < part.heads) {
+                    if (turns) turn(x0[i], x1[i]);
+                    store_chunk<T, V>(dst + (long long)h * part.dst_head + e0, x0[i]);
+                    store_chunk<T, V>(dst + (long long)h * part.dst_head + e1, x1[i]);
+                }
+            }
         }
-        head -= part.heads;
+        // the first of this thread's heads in the next part: they go on in steps of head_groups
+        head = first - part.heads + (first < part.heads ? (part.heads - first + a.head_groups - 1) / a.head_groups * a.head_groups : 0);
     }
 }
 
@@ -138,7 +158,7 @@ int launch_chunks(RopeArgs &a, cudaStream_t st) {
     a.chunks = a.head_dim / (2 * V);
     const int heads = a.part[0].heads + a.part[1].heads + a.part[2].heads;
     // Heads per thread: one as long as that leaves the machine with threads to spare; up to eight share a sine and cosine beyond.
-    const size_t one_each = (size_t)a.tokens * a.chunks * heads, room = (size_t)sm_count() * 2048;
+    const size_t one_each = (size_t)a.tokens * a.chunks * heads, room = (size_t)sm_count() * 1024;
     int per = (int)(one_each / room);
     per = per < 1 ? 1 : (per > 8 ? 8 : per);
     a.head_groups = (heads + per - 1) / per;
