@@ -40,6 +40,7 @@ typedef unsigned long long u64;
 constexpr int SM_NT = 1024, SM_WARPS = SM_NT / 32;
 constexpr int BINS = SM_NT;             // steps of a histogram; what is behind the last counts as one more
 constexpr int EACH = 2, LIST = EACH * SM_NT;  // tokens that are sorted, and of those a thread's
+constexpr int HANDFUL = 192;
 constexpr int MAX_CLUSTER = 8;
 constexpr float STEPS = 64.0f;          // histogram steps per unit of (top - x) / t
 constexpr float MOST = 3.4028234663852886e38f;
@@ -345,11 +346,10 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
         const u64 w = r.weight(x);
         return w >= least ? w : 0;
     };
-    // a logit below those of the steps up to this one, whatever was rounded
-    const double width = (double)t / STEPS;
-    auto edge = [&](int step) {
-        return step < 2 * BINS ? __double2float_rd((double)r.top - (step + 1) * width - (0.01 * width + 1e-6 * fabs((double)r.top))) : -INFINITY;
-    };
+    // a logit below those of the steps up to this one, and one above those from this one on, whatever was rounded
+    const float width = t / STEPS, slack = 0.01f * width + 1e-6f * fabsf(r.top);
+    auto edge = [&](int step) { return step < 2 * BINS ? r.top - (step + 1) * width * 1.00001f - slack : -INFINITY; };
+    auto upper_edge = [&](int step) { return step ? fminf(r.top - step * width * 0.99999f + slack, r.top) : r.top; };
     auto sums_command = [&](u64 cut) {
         Command c{};
         c.op = OP_SUMS; c.cut = cut;
@@ -526,7 +526,49 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
                 const unsigned listed = s.listed;
                 if (!tried) {  // all tokens up to the step that the first filter ends in
                     tried = true;
-                    if (listed <= LIST) {
+                    if (listed <= HANDFUL) {
+                        // A handful: everybody's place among the others, the weights before it and up to it in order of index are counted
+                        // out, by as many threads a token as there are; sorting takes longer, step after step.
+                        const int have = (int)listed;
+                        int parts = SM_NT / 32;
+                        while (SM_NT / parts < have) parts >>= 1;
+                        const int i = tid / parts;
+                        u64 *weight = s.taken, *stays = s.taken + HANDFUL;
+                        if (tid < have) weight[tid] = r.weight(logit_of(s.list[tid]));
+                        __syncthreads();
+                        const u64 place = i < have ? s.list[i] : 0, w = i < have ? weight[i] : 0;
+                        u64 before = 0;
+                        int rank_of = 0;
+                        for (int j = tid % parts; j < have; j += parts)
+                            if (s.list[j] > place) {
+                                before += weight[j];
+                                ++rank_of;
+                            }
+                        for (int o = parts / 2; o; o >>= 1) {
+                            before += __shfl_xor_sync(0xffffffffu, before, o);
+                            rank_of += __shfl_xor_sync(0xffffffffu, rank_of, o);
+                        }
+                        const bool asks = i < have && tid % parts == 0;
+                        if (asks && by_count && rank_of == min(k, have) - 1) s.found_q = before + w;  // what top-k leaves
+                        __syncthreads();
+                        const u64 q = quota(by_count ? s.found_q : whole);
+                        const bool kept_one = (!by_count || rank_of < k) && !(by_weight && before >= q) && w >= least;
+                        if (asks) stays[i] = kept_one ? w : 0;
+                        __syncthreads();
+                        u64 up = 0, all = 0;
+                        for (int j = tid % parts; j < have; j += parts) {
+                            const u64 other = stays[j];
+                            all += other;
+                            if (index_of(s.list[j]) <= index_of(place)) up += other;
+                        }
+                        for (int o = parts / 2; o; o >>= 1) {
+                            up += __shfl_xor_sync(0xffffffffu, up, o);
+                            all += __shfl_xor_sync(0xffffffffu, all, o);
+                        }
+                        const u64 target = draw_at(all);
+                        if (asks && kept_one && up - w <= target && target < up) a.tokens[row] = index_of(place);
+                        c.op = OP_LEAVE;
+                    } else if (listed <= LIST) {
                         sort_list(s, (int)listed);
                         u64 place[EACH], w[EACH], own = 0;
 #pragma unroll
@@ -635,7 +677,7 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
                         c.upto = -1;
                         c.base = 0;
                         c.floor = edge(c.step);
-                        const float above = c.step ? fminf(__double2float_ru((double)r.top - c.step * width + (0.01 * width + 1e-6 * fabs((double)r.top))), r.top) : r.top;
+                        const float above = upper_edge(c.step);
                         const unsigned high = order_of(above), low = order_of(c.floor);
                         const int same = c.floor <= above ? __clz(high ^ low) : 0;
                         c.shift = PLACE_BITS - same;
