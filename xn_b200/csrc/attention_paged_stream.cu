@@ -447,77 +447,114 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
 }
 
 // Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
-// of the CTAs behind it.  A thread holds four columns of AT rows at once; SLICES groups of threads share a row's records.
+// of the CTAs behind it.  A thread holds four columns of AT rows at once, a group of HD / 4 threads the rows.  The groups of a block
+// take rows of their own where an item has few records, and share the records of the same rows where it has many (a long context of
+// few rows has one from every CTA: read one after another, 74 of them took 70 us); records are read a few at a time, before it is known
+// whether they are there.
 constexpr int MERGE_NT = 256;
-template <typename T, int HD, int SLICES, int AT>
+template <typename T, int HD, int AT, bool ALWAYS_SHARED>
 __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
-    constexpr int LANES = HD / 4, ROWS = MERGE_NT / LANES / SLICES;
-    __shared__ float sm[ROWS][SLICES], sl[ROWS][SLICES];
-    __shared__ float4 so[ROWS][SLICES][LANES];
+    constexpr int LANES = HD / 4, GROUPS = MERGE_NT / LANES;
+    __shared__ float sm[GROUPS][AT], sl[GROUPS][AT];
+    __shared__ float4 so[GROUPS][AT][LANES];
     dependent_begin();
     const PartNote *notes = static_cast<const PartNote *>(a.ws);
     const PartNote n = notes[blockIdx.x];
     if (n.last == 0) return;
-    const int in_block = threadIdx.x / (LANES * SLICES), slice = threadIdx.x / LANES % SLICES, lane = threadIdx.x % LANES;
+    const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
-    float m[AT], l[AT];
-    float4 o[AT];
-    int rows[AT], item_rows[AT];
-#pragma unroll
-    for (int i = 0; i < AT; ++i) {
-        const int row = (blockIdx.y * AT + i) * ROWS + in_block, item_row = n.tile_row + (row >> 7) * used + (row & 127);
-        const bool real = row < rec_rows && (row & 127) < used && item_row < n.rows;
-        rows[i] = real ? row : -1;
-        item_rows[i] = item_row;
-        m[i] = -INFINITY;
-        l[i] = 0.0f;
-        o[i] = make_float4(0, 0, 0, 0);
-    }
-    auto join = [&](int i, float rm, float rl, const float4 &ro) {
-        const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
-        const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
-        l[i] = l[i] * w0 + rl * w1;
-        o[i].x = o[i].x * w0 + ro.x * w1;
-        o[i].y = o[i].y * w0 + ro.y * w1;
-        o[i].z = o[i].z * w0 + ro.z * w1;
-        o[i].w = o[i].w * w0 + ro.w * w1;
-        m[i] = mn;
-    };
-    for (int c = blockIdx.x + slice; c <= n.last; c += SLICES) {
-        if (c > (int)blockIdx.x && !notes[c].joined) continue;  // a share in which no key block of the item begins
-        const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-        float rm[AT], rl[AT];
-        float4 ro[AT];
+    const bool shared = ALWAYS_SHARED || n.last - (int)blockIdx.x >= GROUPS;
+    const int slices = shared ? GROUPS : 1, slice = shared ? group : 0;
+    // the block's rows: AT of every group, or AT of all groups at a time
+    constexpr int BLOCK_ROWS = ALWAYS_SHARED ? AT : GROUPS * AT;
+    const int block_rows = min(BLOCK_ROWS, rec_rows - (int)blockIdx.y * BLOCK_ROWS);
+    for (int r0 = shared ? 0 : group * AT; r0 < block_rows; r0 += shared ? AT : block_rows) {
+        float m[AT], l[AT];
+        float4 o[AT];
+        int rows[AT], item_rows[AT];
+        bool any = false;
 #pragma unroll
         for (int i = 0; i < AT; ++i) {
-            const int row = max(rows[i], 0);  // a row that nobody has is not written
-            rm[i] = rows[i] >= 0 ? rec[rec_rows * HD + row] : -INFINITY;
-            rl[i] = rows[i] >= 0 ? rec[rec_rows * HD + rec_rows + row] : 0.0f;
-            ro[i] = rows[i] >= 0 ? reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane] : make_float4(0, 0, 0, 0);
+            const int row = blockIdx.y * BLOCK_ROWS + r0 + i, item_row = n.tile_row + (row >> 7) * used + (row & 127);
+            const bool real = r0 + i < block_rows && (row & 127) < used && item_row < n.rows;
+            any |= real;
+            rows[i] = real ? row : -1;
+            item_rows[i] = item_row;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+            o[i] = make_float4(0, 0, 0, 0);
+        }
+        if (!any) continue;  // the same for all groups that share them
+        auto join = [&](int i, float rm, float rl, const float4 &ro) {
+            const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
+            const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
+            l[i] = l[i] * w0 + rl * w1;
+            o[i].x = o[i].x * w0 + ro.x * w1;
+            o[i].y = o[i].y * w0 + ro.y * w1;
+            o[i].z = o[i].z * w0 + ro.z * w1;
+            o[i].w = o[i].w * w0 + ro.w * w1;
+            m[i] = mn;
+        };
+        constexpr int AHEAD = ALWAYS_SHARED ? 4 : 2;
+        for (int c0 = blockIdx.x + slice; c0 <= n.last; c0 += AHEAD * slices) {
+            int there[AHEAD];
+            float rm[AHEAD][AT], rl[AHEAD][AT];
+            float4 ro[AHEAD][AT];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int c = min(c0 + k * slices, n.last);
+                const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
+                // not there: a share in which no key block of the item begins
+                there[k] = c0 + k * slices <= n.last && (c == (int)blockIdx.x || notes[c].joined);
+#pragma unroll
+                for (int i = 0; i < AT; ++i) {
+                    const int row = max(rows[i], 0);
+                    rm[k][i] = rec[rec_rows * HD + row];
+                    rl[k][i] = rec[rec_rows * HD + rec_rows + row];
+                    ro[k][i] = reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+                if (there[k]) {
+#pragma unroll
+                    for (int i = 0; i < AT; ++i)
+                        if (rows[i] >= 0) join(i, rm[k][i], rl[k][i], ro[k][i]);
+                }
+        }
+        if (shared) {  // group g joins and writes the g-th of the rows
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < AT; ++i) {
+                so[group][i][lane] = o[i];
+                if (lane == 0) { sm[group][i] = m[i]; sl[group][i] = l[i]; }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < AT; ++i) {
+                if (i != group % AT || group >= AT) {
+                    rows[i] = -1;
+                    continue;
+                }
+                m[i] = -INFINITY;
+                l[i] = 0.0f;
+                o[i] = make_float4(0, 0, 0, 0);
+                for (int s = 0; s < GROUPS; ++s) join(i, sm[s][i], sl[s][i], so[s][i][lane]);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < AT; ++i) join(i, rm[i], rl[i], ro[i]);
-    }
-    if (SLICES > 1) {
-        static_assert(SLICES == 1 || AT == 1, "a row's slices are joined for one row at a time");
-        so[in_block][slice][lane] = o[0];
-        if (lane == 0) { sm[in_block][slice] = m[0]; sl[in_block][slice] = l[0]; }
-        __syncthreads();
-        if (slice) return;
-        for (int s = 1; s < SLICES; ++s) join(0, sm[in_block][s], sl[in_block][s], so[in_block][s][lane]);
-    }
-#pragma unroll
-    for (int i = 0; i < AT; ++i) {
-        if (rows[i] < 0) continue;
-        const unsigned r = (unsigned)item_rows[i];
-        T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
-                 (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-        const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-        uint2 w;
-        w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
-        w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
-        reinterpret_cast<uint2 *>(dst)[lane] = w;
+        for (int i = 0; i < AT; ++i) {
+            if (rows[i] < 0) continue;
+            const unsigned r = (unsigned)item_rows[i];
+            T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
+                     (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
+            const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+            uint2 w;
+            w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
+            w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
+            reinterpret_cast<uint2 *>(dst)[lane] = w;
+        }
     }
 }
 
@@ -539,13 +576,12 @@ template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream
 }  // namespace
 
 namespace {
-// Few rows may have a record from every CTA: all threads of a block share one row's.  Many rows have a few each.
 template <typename T, int HD> int launch_merge(int rows, int used, const PagedArgs &a, cudaStream_t st) {
-    constexpr int ROWS = MERGE_NT * 4 / HD, AT = 4;
+    constexpr int GROUPS = MERGE_NT * 4 / HD, AT = 2;
     if (rows <= 16)
-        return launch_dependent(paged_merge_kernel<T, HD, ROWS, 1>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
-    return launch_dependent(paged_merge_kernel<T, HD, 1, AT>, dim3((unsigned)a.parts, (unsigned)((rows + ROWS * AT - 1) / (ROWS * AT))), dim3(MERGE_NT),
-                            0, st, a, rows, used);
+        return launch_dependent(paged_merge_kernel<T, HD, 1, true>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
+    return launch_dependent(paged_merge_kernel<T, HD, AT, false>, dim3((unsigned)a.parts, (unsigned)((rows + GROUPS * AT - 1) / (GROUPS * AT))),
+                            dim3(MERGE_NT), 0, st, a, rows, used);
 }
 }  // namespace
 
