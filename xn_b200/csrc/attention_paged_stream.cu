@@ -446,114 +446,133 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
     if (threadIdx.x == 0) static_cast<PartNote *>(a.ws)[blockIdx.x] = said;
 }
 
-// Joins the records of the item that CTA blockIdx.x of the kernel before began and did not end: its record 1 and the records 0
-// of the CTAs behind it.  A thread holds four columns of AT rows at once, a group of HD / 4 threads the rows.  The groups of a block
-// take rows of their own where an item has few records, and share the records of the same rows where it has many (a long context of
-// few rows has one from every CTA: read one after another, 74 of them took 70 us); records are read a few at a time, before it is known
-// whether they are there.
+// Joins the records of the items that begin in one CTA of the kernel before and go on in others: record 1 of the first and the records 0
+// of the CTAs behind it.  A thread holds four columns of AT rows at once, a group of HD / 4 threads the rows.  Where an item has few
+// records, the blocks of its first CTA join it and their groups take rows of their own.  Where it has many (a long context of few rows
+// has one from every CTA), the groups share the records of the same rows, and the blocks of all its CTAs take rows of it; records
+// are read a few at a time, before it is known whether they are there.  64 rows of 2 heads over 30000 keys on the tensor-memory kernel:
+// 99 us with a row's records read one after another, 62 shared among groups, 23 among blocks too.
 constexpr int MERGE_NT = 256;
 template <typename T, int HD, int AT, bool ALWAYS_SHARED>
 __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
     constexpr int LANES = HD / 4, GROUPS = MERGE_NT / LANES;
     __shared__ float sm[GROUPS][AT], sl[GROUPS][AT];
     __shared__ float4 so[GROUPS][AT][LANES];
+    __shared__ int helps;  // the first CTA of the item that goes on here and has many records
+    const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     dependent_begin();
     const PartNote *notes = static_cast<const PartNote *>(a.ws);
-    const PartNote n = notes[blockIdx.x];
-    if (n.last == 0) return;
-    const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    // threads look for an item that goes on here (there is one at most) while the block's own one is joined
+    int found = -1;
+    if (!ALWAYS_SHARED)
+        for (int c = threadIdx.x; c < (int)blockIdx.x; c += MERGE_NT) {
+            const int last = notes[c].last;
+            if (last >= (int)blockIdx.x && last - c >= GROUPS) found = c;
+        }
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
-    const bool shared = ALWAYS_SHARED || n.last - (int)blockIdx.x >= GROUPS;
-    const int slices = shared ? GROUPS : 1, slice = shared ? group : 0;
-    // the block's rows: AT of every group, or AT of all groups at a time
-    constexpr int BLOCK_ROWS = ALWAYS_SHARED ? AT : GROUPS * AT;
-    const int block_rows = min(BLOCK_ROWS, rec_rows - (int)blockIdx.y * BLOCK_ROWS);
-    for (int r0 = shared ? 0 : group * AT; r0 < block_rows; r0 += shared ? AT : block_rows) {
-        float m[AT], l[AT];
-        float4 o[AT];
-        int rows[AT], item_rows[AT];
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < AT; ++i) {
-            const int row = blockIdx.y * BLOCK_ROWS + r0 + i, item_row = n.tile_row + (row >> 7) * used + (row & 127);
-            const bool real = r0 + i < block_rows && (row & 127) < used && item_row < n.rows;
-            any |= real;
-            rows[i] = real ? row : -1;
-            item_rows[i] = item_row;
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-            o[i] = make_float4(0, 0, 0, 0);
-        }
-        if (!any) continue;  // the same for all groups that share them
-        auto join = [&](int i, float rm, float rl, const float4 &ro) {
-            const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
-            const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
-            l[i] = l[i] * w0 + rl * w1;
-            o[i].x = o[i].x * w0 + ro.x * w1;
-            o[i].y = o[i].y * w0 + ro.y * w1;
-            o[i].z = o[i].z * w0 + ro.z * w1;
-            o[i].w = o[i].w * w0 + ro.w * w1;
-            m[i] = mn;
-        };
-        constexpr int AHEAD = ALWAYS_SHARED ? 4 : 2;
-        for (int c0 = blockIdx.x + slice; c0 <= n.last; c0 += AHEAD * slices) {
-            int there[AHEAD];
-            float rm[AHEAD][AT], rl[AHEAD][AT];
-            float4 ro[AHEAD][AT];
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int c = min(c0 + k * slices, n.last);
-                const float *rec = recs + ((size_t)c * 2 + (c == (int)blockIdx.x)) * rec_floats;
-                // not there: a share in which no key block of the item begins
-                there[k] = c0 + k * slices <= n.last && (c == (int)blockIdx.x || notes[c].joined);
-#pragma unroll
-                for (int i = 0; i < AT; ++i) {
-                    const int row = max(rows[i], 0);
-                    rm[k][i] = rec[rec_rows * HD + row];
-                    rl[k][i] = rec[rec_rows * HD + rec_rows + row];
-                    ro[k][i] = reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane];
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k)
-                if (there[k]) {
-#pragma unroll
-                    for (int i = 0; i < AT; ++i)
-                        if (rows[i] >= 0) join(i, rm[k][i], rl[k][i], ro[k][i]);
-                }
-        }
-        if (shared) {  // group g joins and writes the g-th of the rows
+    for (int turn = 0; turn < (ALWAYS_SHARED ? 1 : 2); ++turn) {
+        int first = blockIdx.x;
+        if (turn == 1) {
+            if (!__syncthreads_or(found >= 0)) break;
+            if (found >= 0) helps = found;
             __syncthreads();
+            first = helps;
+        }
+        const PartNote n = notes[first];
+        if (n.last == 0) continue;
+        const bool shared = ALWAYS_SHARED || n.last - first >= GROUPS;
+        const int slices = shared ? GROUPS : 1, slice = shared ? group : 0;
+        // rows: AT of all groups at a time, dealt out to the blocks of the item's CTAs, or AT of every group
+        const int at = ALWAYS_SHARED ? (int)blockIdx.y : shared ? ((int)blockIdx.x - first) * (int)gridDim.y + (int)blockIdx.y
+                                                                 : (int)blockIdx.y * GROUPS + group;
+        const int step = ALWAYS_SHARED || !shared ? rec_rows : (n.last - first + 1) * (int)gridDim.y * AT;
+        for (int r0 = at * AT; r0 < rec_rows; r0 += step) {
+            float m[AT], l[AT];
+            float4 o[AT];
+            int rows[AT], item_rows[AT];
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < AT; ++i) {
-                so[group][i][lane] = o[i];
-                if (lane == 0) { sm[group][i] = m[i]; sl[group][i] = l[i]; }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < AT; ++i) {
-                if (i != group % AT || group >= AT) {
-                    rows[i] = -1;
-                    continue;
-                }
+                const int row = r0 + i, item_row = n.tile_row + (row >> 7) * used + (row & 127);
+                const bool real = row < rec_rows && (row & 127) < used && item_row < n.rows;
+                any |= real;
+                rows[i] = real ? row : -1;
+                item_rows[i] = item_row;
                 m[i] = -INFINITY;
                 l[i] = 0.0f;
                 o[i] = make_float4(0, 0, 0, 0);
-                for (int s = 0; s < GROUPS; ++s) join(i, sm[s][i], sl[s][i], so[s][i][lane]);
             }
-        }
+            if (!any) continue;  // the same for all groups that share them
+            auto join = [&](int i, float rm, float rl, const float4 &ro) {
+                const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
+                const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
+                l[i] = l[i] * w0 + rl * w1;
+                o[i].x = o[i].x * w0 + ro.x * w1;
+                o[i].y = o[i].y * w0 + ro.y * w1;
+                o[i].z = o[i].z * w0 + ro.z * w1;
+                o[i].w = o[i].w * w0 + ro.w * w1;
+                m[i] = mn;
+            };
+            constexpr int AHEAD = ALWAYS_SHARED ? 4 : 2;
+            for (int c0 = first + slice; c0 <= n.last; c0 += AHEAD * slices) {
+                int there[AHEAD];
+                float rm[AHEAD][AT], rl[AHEAD][AT];
+                float4 ro[AHEAD][AT];
 #pragma unroll
-        for (int i = 0; i < AT; ++i) {
-            if (rows[i] < 0) continue;
-            const unsigned r = (unsigned)item_rows[i];
-            T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
-                     (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-            const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-            uint2 w;
-            w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
-            w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
-            reinterpret_cast<uint2 *>(dst)[lane] = w;
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int c = min(c0 + k * slices, n.last);
+                    const float *rec = recs + ((size_t)c * 2 + (c == first)) * rec_floats;
+                    // not there: a share in which no key block of the item begins
+                    there[k] = c0 + k * slices <= n.last && (c == first || notes[c].joined);
+#pragma unroll
+                    for (int i = 0; i < AT; ++i) {
+                        const int row = max(rows[i], 0);
+                        rm[k][i] = rec[rec_rows * HD + row];
+                        rl[k][i] = rec[rec_rows * HD + rec_rows + row];
+                        ro[k][i] = reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                    if (there[k]) {
+#pragma unroll
+                        for (int i = 0; i < AT; ++i)
+                            if (rows[i] >= 0) join(i, rm[k][i], rl[k][i], ro[k][i]);
+                    }
+            }
+            if (shared) {  // group g joins and writes the g-th of the rows
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < AT; ++i) {
+                    so[group][i][lane] = o[i];
+                    if (lane == 0) { sm[group][i] = m[i]; sl[group][i] = l[i]; }
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < AT; ++i) {
+                    if (i != group % AT || group >= AT) {
+                        rows[i] = -1;
+                        continue;
+                    }
+                    m[i] = -INFINITY;
+                    l[i] = 0.0f;
+                    o[i] = make_float4(0, 0, 0, 0);
+                    for (int s = 0; s < GROUPS; ++s) join(i, sm[s][i], sl[s][i], so[s][i][lane]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < AT; ++i) {
+                if (rows[i] < 0) continue;
+                const unsigned r = (unsigned)item_rows[i];
+                T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
+                         (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
+                const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+                uint2 w;
+                w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
+                w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
+                reinterpret_cast<uint2 *>(dst)[lane] = w;
+            }
         }
     }
 }
