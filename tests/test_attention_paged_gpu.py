@@ -277,3 +277,29 @@ def test_the_bound_on_rows_changes_no_result_beyond_rounding(xn, cuda):
     b = Batch(cuda, torch.bfloat16, [(150, 400), (1, 300)], 8, 2, 128, 16)
     for m in (None, 0, 1, 2, 4, 16, 150, 10 ** 6):
         b.check(b.run(xn, max_query=m))
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,heads,kv,hd,window", [(3, 2, 2, 64, 0), (5, 4, 2, 128, 0), (7, 4, 2, 128, 20), (4, 8, 2, 64, 3), (40, 8, 2, 128, 0),
+                                                  (200, 4, 2, 64, 0), (300, 2, 2, 128, 0), (100, 8, 2, 128, 30), (300, 2, 2, 128, 250), (1, 40, 2, 64, 9)])
+def test_what_is_not_finite_stays_with_the_rows_that_see_it(xn, cuda, dtype, n, heads, kv, hd, window):
+    """An infinity or NaN in a key or a value that some of a sequence's rows see: the others get what they get without it."""
+    b = Batch(cuda, DTYPES[dtype], [(n, n + 100), (n, n), (n, 5000 + n)], heads, kv, hd, 16)
+    want = b.run(xn, max_query=n, window=window)
+    b.check(want, window=window)
+    for pool, value in ((b.v, math.nan), (b.v, math.inf), (b.v, -math.inf), (b.k, math.nan)):
+        saved = pool.clone()
+        seen = torch.zeros(b.rows, dtype=torch.bool, device=cuda)
+        for s, (rows, ctx) in enumerate(b.lengths):
+            at = torch.arange(ctx - rows, ctx, device=cuda)  # the last key that each row sees
+            keys = [ctx - 1, ctx - rows // 2, ctx - rows - (window // 2 if window else -1)] if s != 1 else [rows // 2 + 1]
+            for key in keys:
+                key = min(max(key, 0), ctx - 1)
+                pool[int(b.table[s, key // 16]), 0, key % 16, 5] = value
+                seen[int(b.starts[s]):int(b.starts[s]) + rows] |= (key <= at) & ((key > at - window) if window else True)
+        got = b.run(xn, max_query=n, window=window)
+        pool.copy_(saved)
+        mine = got[:, :heads // kv]
+        assert not bool(mine[seen][:, :, 5].isfinite().any())
+        assert torch.equal(mine[~seen], want[~seen][:, :heads // kv])
+        assert torch.equal(got[:, heads // kv:], want[:, heads // kv:])

@@ -11,8 +11,8 @@
 //   O^T += V^T P^T, V's fragments by transposing loads, P^T turned in registers
 // Keys ride the 16-row dimension, rows the 8-column one: with one to eight rows (a token's heads) half of what the other way
 // round would cost, which keeps the products well below the time that the unit's bytes take to arrive.  P is rounded to the
-// element type for the second product (relative 2^-9 of each, as the output's own rounding); scores, maxima, sums and O stay
-// in f32.
+// element type for the second product (half a step, 2^-8 of each in bf16 and 2^-11 in f16, as the output's own rounding); scores,
+// maxima, sums and O stay in f32.
 //
 // A warp that holds the whole of an item writes its rows; parts are joined within the CTA through shared memory, and what
 // crosses CTAs (at most two records of each) by a second kernel.
@@ -246,6 +246,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
         unsigned qf[HD / 16][NT][2];
         float o[HD / 16][NT][4], m[NT][2], l[NT][2];
         int hi_key[NT][2], lo_key[NT][2];
+        int sure_hi = 0, sure_lo = 0;  // the keys that all rows of the item see
         bool fresh = true;
         unsigned long long item_begin = 0;
         int slot = 0;
@@ -254,6 +255,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                 fresh = false;
                 item_begin = cc.pos - (unsigned)cc.unit;
                 const int rows = (int)min((long long)cc.u.s.n * a.group - (long long)cc.tile * TR, (long long)TR);
+                sure_hi = cc.u.s.off + (int)((unsigned)(cc.tile * TR) / (unsigned)a.group);
+                sure_lo = a.window ? cc.u.s.off + (int)((unsigned)(cc.tile * TR + rows - 1) / (unsigned)a.group) - a.window + 1 : 0;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const int rq = nt * 8 + (lane >> 2);  // the row of this lane's Q fragments
@@ -332,6 +335,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[mt][nt][e] *= alpha[nt][e & 1];
+            }
+            // A row of V that some rows see and others do not, and that is not finite, is taken for zeros (a product with the probability 0
+            // would be NaN), and the rows that see it become NaN.  Beyond the context and before all windows it is zeros anyway.
+            const int unit0 = cc.u.base + cc.unit * UNIT;
+            if ((unit0 + UNIT - 1 > sure_hi && sure_hi < cc.u.s.ctx - 1) || (unit0 < sure_lo && cc.u.lo < sure_lo)) {
+                const int key = unit0 + (lane & 15);  // two lanes a key
+                unsigned char *row = ring + slot * STAGE + TILE + (lane & 15) * ROW_BYTES;
+                NotFinite<T> check;
+#pragma unroll
+                for (int i = 0; i < CHUNKS / 2; ++i)
+                    check.see(*reinterpret_cast<const uint4 *>(row + (((lane >> 4) * (CHUNKS / 2) + ((i ^ lane) & (CHUNKS / 2 - 1))) << 4)));
+                unsigned which = __ballot_sync(0xffffffffu, check.any() && (key > sure_hi || key < sure_lo));
+                if (which) {
+                    which = (which | which >> 16) & 0xffffu;
+                    if (which >> (lane & 15) & 1)
+#pragma unroll
+                        for (int i = 0; i < CHUNKS / 2; ++i)
+                            *reinterpret_cast<uint4 *>(row + (((lane >> 4) * (CHUNKS / 2) + ((i ^ lane) & (CHUNKS / 2 - 1))) << 4)) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            for (unsigned k = which; k; k &= k - 1) {
+                                const int bad_key = unit0 + __ffs(k) - 1;
+                                if (bad_key <= hi_key[nt][e] && bad_key >= lo_key[nt][e]) l[nt][e] = NAN;
+                            }
+                }
             }
 #pragma unroll
             for (int mt = 0; mt < HD / 16; ++mt) {

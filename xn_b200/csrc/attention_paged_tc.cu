@@ -12,7 +12,10 @@
 //
 // Pages: a key block is a few TMA boxes of consecutive rows of a page, their page indexes read one block ahead.  Boxes beyond the
 // context are not loaded, keys beyond it are masked, and the rows of V beyond it are overwritten with zeros in shared memory before a
-// product reads them: whatever the page holds there does not matter.
+// product reads them: whatever the page holds there does not matter.  The same is done where a causal or window border runs through
+// the block and a row of V is not finite; rows of the result that see it become NaN, the others are as if it were not there.  Blocks
+// go from the last key down: a causal item's border block comes first, when its V has time to be looked over (measured: 4 us of
+// 68 in a batch of chunks with the border last, none so).
 //
 // Work is counted in key blocks (twice for items of two tiles), all items laid end to end and dealt out evenly to one persistent CTA per
 // SM; what a CTA holds of an item that it shares with its neighbours becomes a record, joined by the merge kernel.  So a long context
@@ -93,6 +96,16 @@ struct Segment {
     int dual;                     // two tiles
     int record;                   // -1: the whole item; otherwise the record that this part of it becomes
 };
+// The keys that all rows of the segment's item see, and the last that any does.
+struct Sure {
+    int lo, hi, last;
+    __device__ __forceinline__ Sure(const TcArgs &a, const Segment &g) {
+        const int end = min(g.tok0 + (1 + g.dual) * a.tile_tokens, g.n);
+        lo = a.p.window ? g.off + end - a.p.window : 0;
+        hi = min(g.ctx - 1, g.off + g.tok0);
+        last = min(g.ctx, g.off + end) - 1;
+    }
+};
 struct Walk {
     int b, head, index;
     u64 pos;  // where the item begins
@@ -135,14 +148,28 @@ struct Walk {
     }
 };
 
+struct Border {  // a block of V that a causal or window border runs through
+    int key0, sure_hi, sure_lo, first, last;  // first, last: the first and last key that any row of the item sees
+    unsigned slot;
+};
 struct TcShared {
-    uint64_t q_full, q_empty, k_full[K_STAGES], k_empty[K_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
+    uint64_t q_full, q_empty, k_full[K_STAGES], k_empty[K_STAGES], v_raw[V_STAGES], v_full[V_STAGES], v_empty[V_STAGES];
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty, red_full, red_empty, seg_full[SEGS], seg_empty[SEGS];
     Segment segs[SEGS];
+    // keys of the segment that some rows see and others do not, and whose values are not finite: those above Sure::hi upwards, those below
+    // Sure::lo downwards (a row's borders lie at most 255 keys from another's)
+    uint32_t bad[SEGS][2][TC_ROWS / 32], any_bad[SEGS];
+    Border border[V_STAGES];
     uint32_t tmem_slot;
     float red_m[2][128], red_l[2][128];
 };
 
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, unsigned parity) {
+    unsigned done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
@@ -197,12 +224,16 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         prefetch_tmap(&map_v);
         mbar_init(&sh.q_full, 1); mbar_init(&sh.q_empty, 1);
         for (int i = 0; i < K_STAGES; ++i) { mbar_init(&sh.k_full[i], 1); mbar_init(&sh.k_empty[i], 1); }
-        for (int i = 0; i < V_STAGES; ++i) { mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
+        for (int i = 0; i < V_STAGES; ++i) { mbar_init(&sh.v_raw[i], 1); mbar_init(&sh.v_full[i], 1); mbar_init(&sh.v_empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_full[i][0], 4);
             mbar_init(&sh.p_full[i][1], 4);
             mbar_init(&sh.o_full[i], 1);
+        }
+        for (int i = 0; i < SEGS; ++i) {
+            sh.any_bad[i] = 0;
+            for (int w = 0; w < 2 * (TC_ROWS / 32); ++w) sh.bad[i][w >> 3][w & 7] = 0;
         }
         mbar_init(&sh.o_empty, 8);
         mbar_init(&sh.red_full, 8);
@@ -238,25 +269,27 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             unsigned n_block = 0;
             const int pieces = KEYS / args.box;
             const unsigned tile_bytes = (unsigned)(args.tile_tokens * p.group * BKB * H);
-            static_assert(K_STAGES == V_STAGES, "one stage count for both rings");
+            static_assert(K_STAGES == 2 && V_STAGES == 2, "of a ring's blocks one at most waits while another is issued");
+            // stages of V whose blocks a border runs through, issued and not looked over yet, the older one first; -1: none
+            int waits = -1, waits_next = -1;
+            unsigned raw_phase = 0;
             for (unsigned n_seg = 0; ok; ++n_seg) {
                 const unsigned slot = n_seg % SEGS;
                 if (!wait_all(&sh.seg_full[slot], (n_seg / SEGS) & 1u)) break;
                 const Segment g = sh.segs[slot];
-                if (g.nb == 0) break;
                 int page = -1, row = 0;
                 auto fetch = [&](int kb) {  // the page of this lane's piece
                     const int key = kb * KEYS + lane * args.box;
                     page = -1;
                     row = 0;
-                    if (lane < pieces && kb < g.kb0 + g.nb && key < g.ctx) {
+                    if (lane < pieces && kb >= g.kb0 && key < g.ctx) {
                         const int at_page = p.page_shift >= 0 ? key >> p.page_shift : (int)((unsigned)key / (unsigned)p.page_size);
                         row = key - at_page * p.page_size;
                         page = p.table[(long long)g.b * p.table_stride + at_page];
                     }
                 };
-                fetch(g.kb0);
-                if (keys) {  // while the first page's index is on its way
+                fetch(g.kb0 + g.nb - 1);
+                if (keys && g.nb) {  // while the first page's index is on its way
                     ok = wait_all(&sh.q_empty, (n_seg & 1u) ^ 1u);
                     if (!ok) break;
                     if (elect_one()) {
@@ -267,14 +300,62 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                                 tma_load_3d(sQ + t * STAGE + h * HALF, &map_q, h * 64, g.head * p.group, g.row0 + t * args.tile_tokens, &sh.q_full);
                     }
                 }
-                for (int kb = g.kb0; kb < g.kb0 + g.nb; ++kb, ++n_block) {
-                    const int used = min(pieces, max(0, (g.ctx - kb * KEYS + args.box - 1) / args.box));
+                const Sure sure(args, g);
+                for (int j = 0; ok;) {
+                    if (waits < 0) {
+                        waits = waits_next;
+                        waits_next = -1;
+                    }
+                    if (j == g.nb && (waits < 0 || g.nb)) break;
+                    const unsigned n = n_block + (unsigned)j, stage = n % K_STAGES, parity = ((n / K_STAGES) & 1u) ^ 1u;
+                    uint64_t *room = keys ? &sh.k_empty[stage] : &sh.v_empty[stage];
+                    // looked over as soon as it is there, or nothing else can be done
+                    if (waits >= 0 && (j == g.nb || waits_next >= 0 ||
+                                       __any_sync(0xffffffffu, mbar_test(&sh.v_raw[waits], raw_phase >> waits & 1u) || !mbar_test(room, parity)))) {
+                        // Rows of V that no row of the item sees become zeros, and so do those that some see and others do not, if they are not
+                        // finite: a product with the probability 0 would be NaN.  This warp has the time for it, while the next loads
+                        // are on their way.
+                        ok = wait_all(&sh.v_raw[waits], raw_phase >> waits & 1u);
+                        if (!ok) break;
+                        raw_phase ^= 1u << waits;
+                        const Border e = sh.border[waits];
+                        // rows [0, below) and [above, KEYS)
+                        const int below = min(max(e.sure_lo - e.key0, 0), KEYS), above = min(max(e.sure_hi + 1 - e.key0, below), KEYS);
+#pragma unroll 1
+                        for (int i = lane; i < below + KEYS - above; i += 32) {
+                            const int r = i < below ? i : above + i - below, key = e.key0 + r;
+                            unsigned char *vrow = sV + waits * STAGE + r * BKB;
+                            bool clear = key > e.last || key < e.first;
+                            if (!clear) {
+                                NotFinite<T> check;
+#pragma unroll 8
+                                for (int c = 0; c < H * 8; ++c)  // lanes in turned order: eight rows' pieces cover all banks
+                                    check.see(*reinterpret_cast<const uint4 *>(vrow + (c >> 3) * HALF + ((c ^ r) & 7) * 16));
+                                clear = check.any();
+                                if (clear) {
+                                    const int side = key > e.sure_hi ? 0 : 1, at = side ? e.sure_lo - 1 - key : key - e.sure_hi - 1;
+                                    atomicOr(&sh.bad[e.slot][side][at >> 5], 1u << (at & 31));
+                                    sh.any_bad[e.slot] = 1;
+                                }
+                            }
+                            if (clear)
+#pragma unroll
+                                for (int c = 0; c < H * 8; ++c)
+                                    *reinterpret_cast<uint4 *>(vrow + (c >> 3) * HALF + ((c ^ r) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.v_full[waits]);
+                        waits = -1;
+                        continue;
+                    }
+                    const int kb = g.kb0 + g.nb - 1 - j, used = min(pieces, max(0, (g.ctx - kb * KEYS + args.box - 1) / args.box));
                     const int now_page = page, now_row = row;
-                    fetch(kb + 1);
-                    const unsigned stage = n_block % K_STAGES, parity = ((n_block / K_STAGES) & 1u) ^ 1u;
-                    uint64_t *full = keys ? &sh.k_full[stage] : &sh.v_full[stage];
-                    ok = wait_all(keys ? &sh.k_empty[stage] : &sh.v_empty[stage], parity);
+                    fetch(kb - 1);
+                    ok = wait_all(room, parity);
                     if (!ok) break;
+                    const bool border = !keys && (kb * KEYS + KEYS - 1 > sure.hi || kb * KEYS < sure.lo);
+                    uint64_t *full = keys ? &sh.k_full[stage] : border ? &sh.v_raw[stage] : &sh.v_full[stage];
                     unsigned char *dst = (keys ? sK : sV) + stage * STAGE;
                     if (elect_one()) mbar_expect_tx(full, (unsigned)(used * args.box * BKB * H));
                     for (int i = 0; i < used; ++i) {
@@ -284,7 +365,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                             for (int h = 0; h < H; ++h) tma_load_4d(dst + h * HALF + i * args.box * BKB, map, h * 64, rw, g.head, pg, full);
                         }
                     }
+                    if (border) {
+                        (waits < 0 ? waits : waits_next) = (int)stage;
+                        if (lane == 0) sh.border[stage] = Border{kb * KEYS, sure.hi, sure.lo, g.lo, sure.last, slot};
+                        __syncwarp();
+                    }
+                    ++j;
                 }
+                if (g.nb == 0) break;
+                n_block += (unsigned)g.nb;
                 if (lane == 0) mbar_arrive(&sh.seg_empty[slot]);
             }
         } else if (warp == 2) {
@@ -369,6 +458,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const unsigned slot = n_seg % SEGS;
                     if (!mbar_wait(&sh.seg_empty[slot], ((n_seg / SEGS) & 1u) ^ 1u, args.wait)) break;
                     sh.segs[slot] = g;
+                    if (sh.any_bad[slot]) {
+                        sh.any_bad[slot] = 0;
+                        for (int i = 0; i < 2 * (TC_ROWS / 32); ++i) sh.bad[slot][i >> 3][i & 7] = 0;
+                    }
                     mbar_arrive(&sh.seg_full[slot]);
                     if (!more) break;
                 }
@@ -489,7 +582,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int tile_rows = args.tile_tokens * p.group;
         const int r_token = r / p.group, r_head = r % p.group;
         bool ok = true;
-        unsigned n_block = 0, n_mine = 0, n_split = 0;
+        unsigned n_mine = 0, n_split = 0;
         // The first turn is a dry one, with nothing to wait for and nothing written: it brings the code into the instruction cache while the
         // first segment, its keys and its scores are on their way (cold, a first block took 5000 to 9000 cycles instead of 3500).
         bool dry = true;
@@ -497,7 +590,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const unsigned slot = n_seg % SEGS;
             if (!dry && !wait_all(&sh.seg_full[slot], (n_seg / SEGS) & 1u)) break;
             const Segment g = dry ? Segment{1, 0, 0, 0, 0, 0, 1, KEYS, 0, 0, 1, -1} : sh.segs[slot];
-            const int nb = g.nb, dual = g.dual, ctx = g.ctx, lo = g.lo, kb0 = g.kb0;
+            const int nb = g.nb, dual = g.dual, ctx = g.ctx, kb0 = g.kb0;
             if (nb == 0) break;
             const int tok = g.tok0 + (dual ? t * args.tile_tokens : 0) + r_token;
             const bool real = r < tile_rows && tok < g.n && !dry;
@@ -507,30 +600,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             float m = real ? -INFINITY : 0.0f;  // rows of nobody never move their reference
             u64 l2[2] = {0, 0};
             bool begun = false;
-            for (int j = 0; j < nb; ++j, ++n_block) {
+            for (int j = 0; j < nb; ++j) {
                 if (!dual && (j & 1) != t) continue;
-                const int key0 = (kb0 + j) * KEYS;
+                const int key0 = (kb0 + nb - 1 - j) * KEYS;
                 if (!dry) {
                     ok = wait_all(&sh.s_full[t], n_mine & 1u);
                     if (!ok) break;
                     ++n_mine;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                // rows of V that no row of the item sees become zeros, by the tile whose product reads the stage first
-                if ((key0 + KEYS > ctx || key0 < lo) && (t == 0 || !dual) && !dry) {
-                    const unsigned vs = n_block % V_STAGES;
-                    ok = wait_all(&sh.v_full[vs], (n_block / V_STAGES) & 1u);
-                    if (!ok) break;
-                    const int key = key0 + r;
-                    if (key >= ctx || key < lo) {
-#pragma unroll
-                        for (int h = 0; h < H; ++h)
-#pragma unroll
-                            for (int i = 0; i < BKB / 16; ++i)
-                                *reinterpret_cast<uint4 *>(sV + vs * STAGE + h * HALF + r * BKB + i * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
                 if (any_real) {
                     uint32_t v[4][32];
 #pragma unroll
@@ -619,9 +697,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 ok = ok && wait_all(&sh.red_full, turn);
                 const float m0 = sh.red_m[0][r], m1 = sh.red_m[1][r];
                 mm = fmaxf(m0, m1);
-                w0 = m0 == -INFINITY ? 0.0f : exp2_fast((m0 - mm) * p.c);
-                w1 = m1 == -INFINITY || nb == 1 ? 0.0f : exp2_fast((m1 - mm) * p.c);
-                l = (w0 == 0.0f ? 0.0f : w0 * sh.red_l[0][r]) + (w1 == 0.0f ? 0.0f : w1 * sh.red_l[1][r]);
+                const float l0 = sh.red_l[0][r], l1 = sh.red_l[1][r];
+                w0 = l0 == 0.0f ? 0.0f : exp2_fast((m0 - mm) * p.c);  // nothing seen: 0; nothing but NaN: NaN
+                w1 = l1 == 0.0f ? 0.0f : exp2_fast((m1 - mm) * p.c);
+                l = w0 * l0 + w1 * l1;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.red_empty);
             }
@@ -630,6 +709,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (ok && !dry && (!dual || t == 1)) ok = wait_all(&sh.o_full[1], n_seg & 1u);
             if (ok) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (!dry && sh.any_bad[slot]) {
+                    const Sure sure(args, g);
+                    for (int i = 0; i < 2 * TC_ROWS; ++i) {  // a key that the row sees was taken for zeros
+                        const int key = i < TC_ROWS ? sure.hi + 1 + i : sure.lo - 1 - (i - TC_ROWS);
+                        if ((sh.bad[slot][i >> 8][(i & 255) >> 5] >> (i & 31) & 1) && key <= horizon && key >= low) l = NAN;
+                    }
+                }
                 const bool empty = l == 0.0f;
                 const float inv = empty ? 0.0f : 1.0f / l;
                 // Columns of the row that this thread reads: all of its tile's accumulator, or half of both.  32 at a time go through shared
@@ -691,7 +777,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (lane == 0 && !dry) mbar_arrive(&sh.seg_empty[slot]);
             }
             if (dry) {
-                n_block = 0;
                 asm volatile("griddepcontrol.wait;" ::: "memory");  // from here on memory that earlier kernels may use is written
             }
         }

@@ -107,6 +107,20 @@ template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float x, fl
     const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const unsigned *>(&h);
 }
+// Whether an infinity or NaN is among the elements seen: a sum of their products with 0 is NaN then, and 0 otherwise.
+template <typename T> struct NotFinite {
+    typedef std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162> Pair;
+    unsigned sum[4] = {0, 0, 0, 0};
+    __device__ __forceinline__ void see(const uint4 &x) {
+        const unsigned v[4] = {x.x, x.y, x.z, x.w}, zero = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Pair r = __hfma2(*reinterpret_cast<const Pair *>(&v[i]), *reinterpret_cast<const Pair *>(&zero), *reinterpret_cast<const Pair *>(&sum[i]));
+            sum[i] = *reinterpret_cast<const unsigned *>(&r);
+        }
+    }
+    __device__ __forceinline__ bool any() const { return ((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0; }
+};
 __device__ __forceinline__ float exp2_fast(float x) {  // relative error about 2^-22; 0 for -inf
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
