@@ -149,3 +149,22 @@ def test_uniform_out_of_range_draws_a_kept_token(xn, cuda):
 @pytest.mark.gpu
 def test_no_rows(xn, cuda):
     assert xn.sample(torch.zeros(0, 10, device=cuda), torch.zeros(0, device=cuda)).shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [300, 9000, 128001])
+def test_top_p_wherever_its_border_lies(xn, cuda, vocab):
+    """Borders among the likeliest tokens, far down, between clumps of tokens and in the middle of one."""
+    rows = 24
+    g = torch.Generator(device=cuda).manual_seed(vocab + 1)
+    n = lambda s: torch.randn(rows, vocab, generator=g, device=cuda) * s  # noqa: E731
+    clumps = torch.randint(0, 5, (rows, vocab), generator=g, device=cuda).float() * 0.7
+    p = torch.cat([torch.linspace(0.02, 0.98, rows - 8, device=cuda),
+                   torch.tensor([1e-9, 1e-30, 0.0, -1.0, 0.999, 0.99999, 1 - 2.0 ** -24, 0.5], device=cuda)])
+    u = torch.rand(rows, generator=g, device=cuda)
+    steep, two = n(1.0) * 30, n(0.01)
+    two[:, ::3] -= 9.0
+    for x in (n(0.02), n(3.0), steep, clumps, clumps + n(1e-5), clumps + n(0.003), two, two - 300 * (n(1.0) > 1.5).float()):
+        check(xn, x, u, top_p=p)
+        check(xn, x, u, top_p=p, min_p=torch.full((rows,), 0.2, device=cuda), temperature=0.2 + u)
+    check(xn, n(1e-37), u, top_p=p, temperature=torch.full((rows,), 1e-38, device=cuda))
