@@ -390,7 +390,7 @@ int xn_mm_rope(xn_dtype dtype, void *dst, size_t dst_token_stride, size_t dst_he
 /* The new tokens of a batch go into the cache: k is turned like xn_mm_rope and written to its slot, v is written as it is, and
  * q (when q_dst is not null: contiguous (tokens, heads, head_dim)) is turned on the way -- one launch over the rows of the fused
  * projection.  freqs null: nothing is turned.  A slot outside [0, num_pages * page_size) stores nothing (padding);
- * the slots of one call are distinct.  What else the pools hold stays as it is. */
+ * the slots of one call are distinct, and k, v and q lie outside the pools.  What else the pools hold stays as it is. */
 int xn_mm_paged_append(xn_dtype dtype, void *k_pages, void *v_pages, size_t page_stride, size_t head_stride, size_t row_stride,
                        size_t num_pages, size_t page_size, const void *k, size_t k_token_stride, size_t k_head_stride, const void *v,
                        size_t v_token_stride, size_t v_head_stride, const int64_t *slots, size_t tokens, size_t kv_heads,
@@ -407,8 +407,8 @@ int xn_mm_paged_append(xn_dtype dtype, void *k_pages, void *v_pages, size_t page
  * Lengths and indexes are device memory that the host does not see: a length is bounded by the tensors, and a page index outside
  * [0, num_pages) reads as a page of zeros.  What pages hold beyond a sequence's context is never used.  A key or value inside
  * the context that is not finite makes the rows that see it so (maybe in all of the head's elements), and no others.
- * workspace: xn_mm_attention_paged_workspace_bytes(head_dim) bytes of device memory, 256-byte aligned, owned by the
- * caller; calls that may overlap need one each. */
+ * out overlaps none of the other tensors.  workspace: xn_mm_attention_paged_workspace_bytes(head_dim) bytes (a number of the current
+ * device's) of device memory, 256-byte aligned, owned by the caller; calls that may overlap need one each. */
 size_t xn_mm_attention_paged_workspace_bytes(size_t head_dim);
 int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token_stride, size_t out_head_stride, const void *q,
                           size_t q_token_stride, size_t q_head_stride, size_t tokens, size_t heads, const void *k_pages,

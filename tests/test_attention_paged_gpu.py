@@ -303,3 +303,21 @@ def test_what_is_not_finite_stays_with_the_rows_that_see_it(xn, cuda, dtype, n, 
         assert not bool(mine[seen][:, :, 5].isfinite().any())
         assert torch.equal(mine[~seen], want[~seen][:, :heads // kv])
         assert torch.equal(got[:, heads // kv:], want[:, heads // kv:])
+
+
+@pytest.mark.parametrize("n", [1, 5, 70])
+def test_broadcast_queries_and_pools(xn, cuda, n):
+    """Dimensions of stride 0 are read like any other: one query for all heads or tokens, one key head or page for all."""
+    b = Batch(cuda, torch.bfloat16, [(n, 150), (n, 90), (n, n)], 8, 2, 64, 16)
+    k, v = (torch.nan_to_num(t) for t in (b.k, b.v))
+    run = lambda q, k, v: xn.attention_paged(q, k, v, b.table, b.context, b.scale, query_starts=b.starts, max_query=n)  # noqa: E731
+    for q in (b.q[:, :1].expand_as(b.q), b.q[:1].expand_as(b.q), b.q[:1, :1].expand_as(b.q)):
+        wide = Batch.__new__(Batch)
+        wide.__dict__.update(b.__dict__, q=q.contiguous(), k=k, v=v)
+        wide.check(run(q, k, v))
+    for kk, vv in ((k[:, :1].expand_as(k), v[:, :1].expand_as(v)), (k[3:4].expand_as(k), v[3:4].expand_as(v))):
+        wide = Batch.__new__(Batch)
+        wide.__dict__.update(b.__dict__, k=kk.contiguous(), v=vv.contiguous())
+        wide.check(run(b.q, kk, vv))
+    assert torch.equal(xn.attention_paged(b.q, k, v, b.table[:1].expand_as(b.table), b.context, b.scale, query_starts=b.starts, max_query=n),
+                       xn.attention_paged(b.q, k, v, b.table[:1].expand_as(b.table).contiguous(), b.context, b.scale, query_starts=b.starts, max_query=n))

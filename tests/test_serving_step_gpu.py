@@ -162,3 +162,44 @@ def test_prompts_and_then_token_by_token(xn, cuda, dtype, hd, interleaved, windo
     others = torch.ones(layer.k.shape[0], dtype=torch.bool, device=cuda)
     others[used] = False
     assert bool(layer.k[others].isnan().all()) and bool(layer.v[others].isnan().all())
+
+
+def test_two_streams_at_once(xn, cuda):
+    """Appends and draws of two programs overlap, each on its own stream and tensors, and captured into graphs that are replayed at once."""
+    g = torch.Generator(device=cuda).manual_seed(3)
+    freqs = xn.rope_frequencies(64, device=cuda)
+    programs = []
+    for i in range(2):
+        p = dict(qkv=torch.randn(300, 6, 64, generator=g, device=cuda).bfloat16(), pools=torch.zeros(2, 24, 1, 16, 64, device=cuda, dtype=torch.bfloat16),
+                 slots=torch.randperm(24 * 16, generator=g, device=cuda)[:300], at=torch.arange(300, device=cuda) * (7 + i),
+                 logits=torch.randn(20 + 30 * i, 30000, generator=g, device=cuda) * 3, top_p=torch.full((20 + 30 * i,), 0.9, device=cuda))
+        p["u"] = torch.rand(len(p["logits"]), generator=g, device=cuda)
+        programs.append(p)
+
+    def run(p):
+        q = xn.paged_append_(*p["pools"], p["qkv"][:, 4:5], p["qkv"][:, 5:], p["slots"], q=p["qkv"][:, :4], positions=p["at"], freqs=freqs)
+        return q, xn.rope(q, p["at"], -freqs), p["pools"].clone(), xn.sample(p["logits"], p["u"], top_p=p["top_p"])
+
+    want = [run(p) for p in programs]
+    for p, w in zip(programs, want):
+        # turned back: two roundings of at most half a step of the pair's length
+        length = p["qkv"][:, :4].double().unflatten(-1, (2, 32)).norm(dim=-2, keepdim=True).expand(-1, -1, 2, -1).flatten(-2)
+        assert bool(((w[1].double() - p["qkv"][:, :4].double()).abs() <= length * (2.5 * torch.finfo(torch.bfloat16).eps)).all())
+    streams = [torch.cuda.Stream() for _ in programs]
+    graphs, replayed = [torch.cuda.CUDAGraph() for _ in programs], []
+    torch.cuda.synchronize()
+    for p, graph in zip(programs, graphs):
+        with torch.cuda.graph(graph):
+            replayed.append(run(p))
+    for _ in range(5):
+        got = []
+        for p, s in zip(programs, streams):
+            with torch.cuda.stream(s):
+                got.append(run(p))
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for w, a, b in zip(want, got, replayed):
+            assert all(torch.equal(x, y) for x, y in zip(w, a)) and all(torch.equal(x, y) for x, y in zip(w, b))
