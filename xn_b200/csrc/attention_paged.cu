@@ -59,7 +59,7 @@ extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token
     if (max_query > tokens || max_query == 0) max_query = tokens;
     // rows: query heads of one key head times the new tokens.  The streaming kernel reads the keys once for 16 of them and has its first
     // loads on their way sooner; the tensor-memory kernel reads them once for 256.  Measured at head_dim 128 (streaming / tensor
-    // memory, us): 8 rows of 4 key heads, 4 x 30000 keys 30 / 35, 16 x 3000 18 / 24; 16 rows of 2, 4 x 30000 24 / 25, 16 x 3000
+    // memory, us): 8 rows of 4 key heads, 4 x 30000 keys 30 / 36, 16 x 3000 18 / 25; 16 rows of 2, 4 x 30000 24 / 27, 16 x 3000
     // 20 / 21, 1 x 1000 13 / 16; 32 rows of 4, 4 x 30000 53 / 37, 16 x 3000 37 / 25, 1 x 1000 13 / 18.
     const size_t rows = max_query * (heads / kv_heads);
     if (rows > 16 && paged_tc_fits(a)) return launch_paged_tc(dtype, (int)head_dim, a, (cudaStream_t)stream);

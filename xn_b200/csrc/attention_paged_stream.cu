@@ -478,17 +478,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
 }
 
 // Joins the records of the items that begin in one CTA of the kernel before and go on in others: record 1 of the first and the records 0
-// of the CTAs behind it.  A thread holds four columns of AT rows at once, a group of HD / 4 threads the rows.  Where an item has few
-// records, the blocks of its first CTA join it and their groups take rows of their own.  Where it has many (a long context of few rows
-// has one from every CTA), the groups share the records of the same rows, and the blocks of all its CTAs take rows of it; records
+// of the CTAs behind it.  A thread holds 4 * NV columns of AT rows at once, a group of HD / (4 * NV) threads the rows.  Where an item has
+// few records, the blocks of its first CTA join it and their groups take rows of their own.  Where it has many (a long context of few
+// rows has one from every CTA), the groups share the records of the same rows, and the blocks of all its CTAs take rows of it; records
 // are read a few at a time, before it is known whether they are there.  64 rows of 2 heads over 30000 keys on the tensor-memory kernel:
-// 99 us with a row's records read one after another, 62 shared among groups, 23 among blocks too.
-constexpr int MERGE_NT = 256;
-template <typename T, int HD, int AT, bool ALWAYS_SHARED>
+// 99 us with a row's records read one after another, 62 shared among groups, 22 among blocks too.  16 columns a thread in that kernel's
+// case (4: twice the instructions for the weights of the records, a batch of chunks 65 to 68 us).
+constexpr int MERGE_NT = 256, MANY_RECORDS = 8;
+template <typename T, int HD, int NV, int AT, bool ALWAYS_SHARED>
 __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
-    constexpr int LANES = HD / 4, GROUPS = MERGE_NT / LANES;
+    constexpr int LANES = HD / (4 * NV), GROUPS = MERGE_NT / LANES, AHEAD = ALWAYS_SHARED ? 4 : 2;
     __shared__ float sm[GROUPS][AT], sl[GROUPS][AT];
-    __shared__ float4 so[GROUPS][AT][LANES];
+    __shared__ float4 so[GROUPS][AT][NV][LANES];
     __shared__ int helps;  // the first CTA of the item that goes on here and has many records
     const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     dependent_begin();
@@ -498,10 +499,27 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
     if (!ALWAYS_SHARED)
         for (int c = threadIdx.x; c < (int)blockIdx.x; c += MERGE_NT) {
             const int last = notes[c].last;
-            if (last >= (int)blockIdx.x && last - c >= GROUPS) found = c;
+            if (last >= (int)blockIdx.x && last - c >= MANY_RECORDS) found = c;
         }
     const size_t rec_floats = part_record_floats(rec_rows, HD);
     const float *recs = part_records(a.ws, a.parts);
+    struct Part {  // of a row
+        float m, l;
+        float4 o[NV];
+    };
+    auto join = [](Part &x, const Part &y) {
+        const float mn = fmaxf(x.m, y.m), ref = mn == -INFINITY ? 0.0f : mn;
+        const float w0 = exp2_fast(x.m - ref), w1 = exp2_fast(y.m - ref);
+        x.l = x.l * w0 + y.l * w1;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            x.o[v].x = x.o[v].x * w0 + y.o[v].x * w1;
+            x.o[v].y = x.o[v].y * w0 + y.o[v].y * w1;
+            x.o[v].z = x.o[v].z * w0 + y.o[v].z * w1;
+            x.o[v].w = x.o[v].w * w0 + y.o[v].w * w1;
+        }
+        x.m = mn;
+    };
     for (int turn = 0; turn < (ALWAYS_SHARED ? 1 : 2); ++turn) {
         int first = blockIdx.x;
         if (turn == 1) {
@@ -512,15 +530,14 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
         }
         const PartNote n = notes[first];
         if (n.last == 0) continue;
-        const bool shared = ALWAYS_SHARED || n.last - first >= GROUPS;
+        const bool shared = ALWAYS_SHARED || n.last - first >= MANY_RECORDS;
         const int slices = shared ? GROUPS : 1, slice = shared ? group : 0;
         // rows: AT of all groups at a time, dealt out to the blocks of the item's CTAs, or AT of every group
         const int at = ALWAYS_SHARED ? (int)blockIdx.y : shared ? ((int)blockIdx.x - first) * (int)gridDim.y + (int)blockIdx.y
                                                                  : (int)blockIdx.y * GROUPS + group;
-        const int step = ALWAYS_SHARED || !shared ? rec_rows : (n.last - first + 1) * (int)gridDim.y * AT;
+        const int step = (int)gridDim.y * AT * (ALWAYS_SHARED ? 1 : shared ? n.last - first + 1 : GROUPS);
         for (int r0 = at * AT; r0 < rec_rows; r0 += step) {
-            float m[AT], l[AT];
-            float4 o[AT];
+            Part mine[AT];
             int rows[AT], item_rows[AT];
             bool any = false;
 #pragma unroll
@@ -530,26 +547,15 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
                 any |= real;
                 rows[i] = real ? row : -1;
                 item_rows[i] = item_row;
-                m[i] = -INFINITY;
-                l[i] = 0.0f;
-                o[i] = make_float4(0, 0, 0, 0);
+                mine[i].m = -INFINITY;
+                mine[i].l = 0.0f;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) mine[i].o[v] = make_float4(0, 0, 0, 0);
             }
             if (!any) continue;  // the same for all groups that share them
-            auto join = [&](int i, float rm, float rl, const float4 &ro) {
-                const float mn = fmaxf(m[i], rm), ref = mn == -INFINITY ? 0.0f : mn;
-                const float w0 = exp2_fast(m[i] - ref), w1 = exp2_fast(rm - ref);
-                l[i] = l[i] * w0 + rl * w1;
-                o[i].x = o[i].x * w0 + ro.x * w1;
-                o[i].y = o[i].y * w0 + ro.y * w1;
-                o[i].z = o[i].z * w0 + ro.z * w1;
-                o[i].w = o[i].w * w0 + ro.w * w1;
-                m[i] = mn;
-            };
-            constexpr int AHEAD = ALWAYS_SHARED ? 4 : 2;
             for (int c0 = first + slice; c0 <= n.last; c0 += AHEAD * slices) {
                 int there[AHEAD];
-                float rm[AHEAD][AT], rl[AHEAD][AT];
-                float4 ro[AHEAD][AT];
+                Part read[AHEAD][AT];
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
                     const int c = min(c0 + k * slices, n.last);
@@ -559,25 +565,29 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
 #pragma unroll
                     for (int i = 0; i < AT; ++i) {
                         const int row = max(rows[i], 0);
-                        rm[k][i] = rec[rec_rows * HD + row];
-                        rl[k][i] = rec[rec_rows * HD + rec_rows + row];
-                        ro[k][i] = reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[lane];
+                        read[k][i].m = rec[rec_rows * HD + row];
+                        read[k][i].l = rec[rec_rows * HD + rec_rows + row];
+#pragma unroll
+                        for (int v = 0; v < NV; ++v) read[k][i].o[v] = reinterpret_cast<const float4 *>(rec + (size_t)row * HD)[v * LANES + lane];
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k)
                     if (there[k]) {
 #pragma unroll
-                        for (int i = 0; i < AT; ++i)
-                            if (rows[i] >= 0) join(i, rm[k][i], rl[k][i], ro[k][i]);
+                        for (int i = 0; i < AT; ++i) {
+                            if (k == 0 && !ALWAYS_SHARED && c0 == first) mine[i] = read[k][i];
+                            else join(mine[i], read[k][i]);
+                        }
                     }
             }
             if (shared) {  // group g joins and writes the g-th of the rows
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < AT; ++i) {
-                    so[group][i][lane] = o[i];
-                    if (lane == 0) { sm[group][i] = m[i]; sl[group][i] = l[i]; }
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) so[group][i][v][lane] = mine[i].o[v];
+                    if (lane == 0) { sm[group][i] = mine[i].m; sl[group][i] = mine[i].l; }
                 }
                 __syncthreads();
 #pragma unroll
@@ -586,10 +596,15 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
                         rows[i] = -1;
                         continue;
                     }
-                    m[i] = -INFINITY;
-                    l[i] = 0.0f;
-                    o[i] = make_float4(0, 0, 0, 0);
-                    for (int s = 0; s < GROUPS; ++s) join(i, sm[s][i], sl[s][i], so[s][i][lane]);
+                    for (int g = 0; g < GROUPS; ++g) {
+                        Part other;
+                        other.m = sm[g][i];
+                        other.l = sl[g][i];
+#pragma unroll
+                        for (int v = 0; v < NV; ++v) other.o[v] = so[g][i][v][lane];
+                        if (g == 0) mine[i] = other;
+                        else join(mine[i], other);
+                    }
                 }
             }
 #pragma unroll
@@ -598,11 +613,14 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
                 const unsigned r = (unsigned)item_rows[i];
                 T *dst = static_cast<T *>(a.out) + (long long)(n.q0 + (int)(r / (unsigned)a.group)) * a.out_token +
                          (long long)(n.head * a.group + (int)(r % (unsigned)a.group)) * a.out_head;
-                const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-                uint2 w;
-                w.x = pack2<T>(o[i].x * inv, o[i].y * inv);
-                w.y = pack2<T>(o[i].z * inv, o[i].w * inv);
-                reinterpret_cast<uint2 *>(dst)[lane] = w;
+                const float inv = mine[i].l == 0.0f ? 0.0f : 1.0f / mine[i].l;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    uint2 w;
+                    w.x = pack2<T>(mine[i].o[v].x * inv, mine[i].o[v].y * inv);
+                    w.y = pack2<T>(mine[i].o[v].z * inv, mine[i].o[v].w * inv);
+                    reinterpret_cast<uint2 *>(dst)[v * LANES + lane] = w;
+                }
             }
         }
     }
@@ -627,11 +645,11 @@ template <typename T, int HD, int NT> int launch_stream(PagedArgs &a, cudaStream
 
 namespace {
 template <typename T, int HD> int launch_merge(int rows, int used, const PagedArgs &a, cudaStream_t st) {
-    constexpr int GROUPS = MERGE_NT * 4 / HD, AT = 2;
+    constexpr int NV = 4, AT = 1, BLOCK = MERGE_NT * 4 * NV / HD * AT;
     if (rows <= 16)
-        return launch_dependent(paged_merge_kernel<T, HD, 1, true>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
-    return launch_dependent(paged_merge_kernel<T, HD, AT, false>, dim3((unsigned)a.parts, (unsigned)((rows + GROUPS * AT - 1) / (GROUPS * AT))),
-                            dim3(MERGE_NT), 0, st, a, rows, used);
+        return launch_dependent(paged_merge_kernel<T, HD, 1, 1, true>, dim3((unsigned)a.parts, (unsigned)rows), dim3(MERGE_NT), 0, st, a, rows, used);
+    return launch_dependent(paged_merge_kernel<T, HD, NV, AT, false>, dim3((unsigned)a.parts, (unsigned)((rows + BLOCK - 1) / BLOCK)), dim3(MERGE_NT),
+                            0, st, a, rows, used);
 }
 }  // namespace
 
