@@ -21,14 +21,14 @@
 //   there are k tokens at least down to the step in which the k-th of those lies; then the tokens up to that step: where they are
 //   few (2048), they are sorted, or counted out, and all filters and the draw are done among them;
 //   with top-p alone, a histogram of rough weights, which says where the border is thought to be; then all weights once, those
-//   above that place and those behind it, and the tokens around it (some hundred), among which the exact border is found;
+//   above that place and those behind it, and the tokens around it (some dozens), among which the exact border is found;
 //   where there are too many tokens, or the border is not where it was thought to be: a histogram of the tokens, or of their exact
 //   weights, the tokens of the step that the filter ends in (split further by the next bits of their 64-bit order while they
 //   are too many), which give the exact end;
 //   the kept weights of every warp's stretch of the row, and the stretch that the draw falls into.
 // Bound: the latency of the passes for few rows; for many, the instructions of the weights, the histogram's additions in shared
-// memory and the reads.  Measured, all in us: one row of 32000 f32, all filters, 20; 24 rows of 50000 bf16 47; 64 rows of 128001
-// f32, top-p, 71 (105 with the exact weights put into the histogram, which took two passes over them); no filter 48.
+// memory and the reads.  Measured, all in us: one row of 32000 f32, all filters, 20; 24 rows of 50000 bf16 35; 64 rows of 128001
+// f32, top-p, 72 (105 with the exact weights put into the histogram, which took two passes over them); no filter 48.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -117,6 +117,7 @@ struct Shared {
     u64 far;                         // behind the histogram; OP_SPLIT: from `lo` on
     u64 ahead;                       // OP_SPLIT: above
     float lo, hi;
+    bool few;
     unsigned listed, found, place;
     u64 found_q;
     int found_bin;
@@ -338,18 +339,18 @@ template <typename T> __device__ __noinline__ u64 first_pass(const View v, int g
     });
     return top > -INFINITY ? place_of(fminf(top, MOST), top_index) : 0;
 }
-// Weights by step in 11 bits of what the step's first token weighs: 2048 (1 - y / 64) for one y of a step behind it, all that 2^20 additions
+// Weights by step in 12 bits of what the step's first token weighs: 4096 (1 - y / 64) for one y of a step behind it, all that 2^20 additions
 // leave room for, and near enough to find where a border lies.
 template <typename T> __device__ __noinline__ void guess_pass(const View v, int g0, int g1) {
     Shared &s = shared();
     const Weigher r(s);
     empty_bins(s);
-    const float fine = 32.0f * r.steps;
+    const float fine = 64.0f * r.steps;
     walk<T, EVERY>(v, g0, g1, 0.0f, [&](int, const float (&x)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int z = __float2int_rz(r.below(x[e]) * fine);
-            atomicAdd(&s.low[min(z >> 5, 2 * BINS - 1)], 2048u - (unsigned)(z & 31));
+            atomicAdd(&s.low[min(z >> 6, 2 * BINS - 1)], 4095u - (unsigned)(z & 63));
         }
     });
 }
@@ -694,9 +695,10 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
 
         // ---- the leader looks at what it found ----
         if (rank == 0 && op == OP_GUESS) {
-            // Cumulated, where the border falls in its step as if the tokens lay evenly in it, and how far to either side it may be: they
-            // lie by chance, so that their number up to a place in the step is off by half the root of their number, and
-            // four times that is looked at, and a few tokens more.
+            // Where the cumulated weights come to 2^-16 of all less than the quota, and where to 2^-16 more: rough weights are off by
+            // 2^-13 each at most, to either side, and their sums by less.  The tokens of a step lie in it by chance, so that their number
+            // up to a place is off by half the root of their number: four times that is looked at, and a few tokens more.  Of a step
+            // with few tokens, or of values of 16 bits, which lie in clumps, all of them are.
             constexpr int MINE = 2 * PER;
             float n[MINE], tokens = 0.0f;
             u64 w[MINE], own = 0;
@@ -706,22 +708,28 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
                 u64 q = 0;
                 for (int o = 0; o < ranks; ++o) q += cluster.map_shared_rank(&s, o)->low[at];
                 if (at == 2 * BINS - 1) q = 0;  // the rest of the row
-                n[e] = (float)q * (1.0f / 2048.0f);
+                n[e] = (float)q * (1.0f / 4096.0f);
                 w[e] = (u64)((float)q * __expf(at * (-1.0f / STEPS)) * 1048576.0f);
                 tokens += n[e];
                 own += w[e];
             }
             ulonglong2 sum = block_scan(s, own);
             float before = (float)block_scan(s, (u64)(tokens + 0.5f)).x;
-            const u64 want = min(max((u64)((double)p * (double)sum.y), 1ull), max(sum.y, 1ull));
+            const u64 want = (u64)((double)p * (double)sum.y), slack_of = sum.y >> 16;
+            const u64 from = want > slack_of ? want - slack_of : 1, to = max(min(want + slack_of, sum.y), (u64)1);
 #pragma unroll
             for (int e = 0; e < MINE; ++e) {
-                if (sum.x < want && want <= sum.x + w[e]) {
-                    const float part = (float)(want - sum.x) / (float)w[e], about = fmaxf(n[e], 1.0f);
-                    const float reach = (2.0f * sqrtf(about) + 4.0f) / about, at = MINE * tid + e + part;
-                    s.hi = at + reach;
-                    // few tokens in all: all of them
-                    s.lo = before + part * about + reach * about <= HANDFUL / 2 ? -INFINITY : at - reach;
+                const float about = fmaxf(n[e], 1.0f), reach = (2.0f * sqrtf(about) + 4.0f) / about;
+                const int at = MINE * tid + e;
+                const bool whole_step = sizeof(T) == 2 || about <= HANDFUL / 3;
+                if (sum.x < from && from <= sum.x + w[e]) {
+                    const float place = at + (float)(from - sum.x) / (float)w[e] - reach;
+                    s.lo = whole_step ? fminf(place, (float)at) : place;
+                }
+                if (sum.x < to && to <= sum.x + w[e]) {
+                    const float part = (float)(to - sum.x) / (float)w[e], place = at + part + reach;
+                    s.hi = whole_step ? fmaxf(place, at + 1.0f) : place;
+                    s.few = before + (whole_step ? 1.0f : part + reach) * about <= HANDFUL / 2;
                 }
                 sum.x += w[e];
                 before += n[e];
@@ -729,7 +737,7 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
             __syncthreads();
             Command c{};
             c.op = OP_SPLIT;
-            c.lo = s.lo;
+            c.lo = s.few ? -INFINITY : s.lo;  // few tokens in all: all of them
             c.hi = s.hi;
             publish(c);
         } else if (rank == 0) {
@@ -771,11 +779,13 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
                 const u64 place = i < have ? s.list[i] : 0, w = i < have ? weight[i] : 0;
                 u64 before = 0;
                 int rank_of = 0;
-                for (int j = tid % parts; j < have; j += parts)
-                    if (s.list[j] > place) {
-                        before += weight[j];
-                        ++rank_of;
-                    }
+#pragma unroll 4
+                for (int j = tid % parts; j < have; j += parts) {
+                    const u64 other = weight[j];
+                    const bool ahead = s.list[j] > place;
+                    before += ahead ? other : 0;
+                    rank_of += ahead;
+                }
                 for (int o = parts / 2; o; o >>= 1) {
                     before += __shfl_xor_sync(0xffffffffu, before, o);
                     rank_of += __shfl_xor_sync(0xffffffffu, rank_of, o);
@@ -795,10 +805,11 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
                     if (asks && kept_one && !missed) atomicAdd(&s.seg[stretch_of(index_of(place))], w);
                 } else if (!missed) {
                     u64 up = 0, all = 0;
+#pragma unroll 4
                     for (int j = tid % parts; j < have; j += parts) {
                         const u64 other = stays[j];
                         all += other;
-                        if (index_of(s.list[j]) <= index_of(place)) up += other;
+                        up += index_of(s.list[j]) <= index_of(place) ? other : 0;
                     }
                     for (int o = parts / 2; o; o >>= 1) {
                         up += __shfl_xor_sync(0xffffffffu, up, o);
