@@ -1,6 +1,9 @@
 """The operators of a serving step as a program runs them: ragged prompts, then token by token, a linear before and after, eagerly on
 a side stream and as a replayed graph; what every operator gave, and the whole cache, against the formulas in 64 bits."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -203,3 +206,33 @@ def test_two_streams_at_once(xn, cuda):
         torch.cuda.synchronize()
         for w, a, b in zip(want, got, replayed):
             assert all(torch.equal(x, y) for x, y in zip(w, a)) and all(torch.equal(x, y) for x, y in zip(w, b))
+
+
+FIRST_IN_A_CAPTURE = """
+import torch, xn_b200 as xn
+d = torch.device("cuda:0")
+g = torch.Generator(device=d).manual_seed(0)
+rand = lambda *s: torch.randn(*s, generator=g, device=d)
+whole = lambda v: torch.tensor(v, dtype=torch.int32, device=d)
+qkv, pools, x = rand(64, 12, 64).bfloat16(), torch.zeros(2, 9, 2, 16, 64, device=d, dtype=torch.bfloat16), rand(4, 40000)
+at, freqs, table = torch.arange(64, device=d), xn.rope_frequencies(64, device=d), torch.arange(9, dtype=torch.int32, device=d)[None]
+u, p, context, starts, one = torch.rand(4, device=d), torch.full((4,), 0.9, device=d), whole([64]), whole([0, 64]), whole([50])
+def step():
+    q = xn.paged_append_(*pools, qkv[:, 8:10], qkv[:, 10:], at, q=qkv[:, :8], positions=at, freqs=freqs)
+    return (q, xn.rope(q, at, freqs), xn.attention_paged(q, *pools, table, context, 0.1, query_starts=starts),
+            xn.attention_paged(q[:1], *pools, table, one, 0.1), xn.sample(x, u, top_p=p))
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+"""
+
+
+def test_the_first_calls_of_a_process_in_a_capture(cuda):
+    """Nothing that a call sets up once is refused while a stream is captured."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0, run.stderr[-2000:]

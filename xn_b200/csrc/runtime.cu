@@ -107,7 +107,11 @@ int wait_ctx(WaitCtx *out) {
         std::lock_guard<std::mutex> lock(g_mu);
         if (!g_status[dev]) {
             void *p = nullptr;
-            XN_CHECK_CUDA(cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable));
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // an allocation is no part of a capture
+            XN_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+            XN_CHECK_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            XN_CHECK_CUDA(e);
             *static_cast<volatile unsigned *>(p) = 0;
             g_status[dev] = static_cast<volatile unsigned *>(p);
         }
