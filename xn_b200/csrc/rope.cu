@@ -18,7 +18,7 @@
 namespace xn {
 namespace {
 
-constexpr int ROPE_NT = 128;  // 256: 13.2 us instead of 11.2 for the f16 append below, the last blocks run longer alone
+constexpr int ROPE_NT = 128;  // 256: 13.2 us instead of 11.2 for the f16 append above, whose last blocks run alone for longer
 
 // One tensor [tokens, heads, head_dim] of the call: where it is read and where it goes.  dst == null marks an unused one.
 struct RopePart {
