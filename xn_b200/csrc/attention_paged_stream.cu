@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
 // Joins the records of the items that begin in one CTA of the kernel before and go on in others: record 1 of the first and the records 0
 // of the CTAs behind it.  A thread holds 4 * NV columns of AT rows at once, a group of HD / (4 * NV) threads the rows.  Where an item has
 // few records, the blocks of its first CTA join it and their groups take rows of their own.  Where it has many (a long context of few
-// rows has one from every CTA), the groups share the records of the same rows, and the blocks of all its CTAs take rows of it; records
+// rows has one from every CTA), several groups share the records of the same rows, and the blocks of all its CTAs take rows of it; records
 // are read a few at a time, before it is known whether they are there.  64 rows of 2 heads over 30000 keys on the tensor-memory kernel:
 // 99 us with a row's records read one after another, 62 shared among groups, 22 among blocks too.  16 columns a thread in that kernel's
 // case (4: twice the instructions for the weights of the records, a batch of chunks 65 to 68 us).
@@ -488,6 +488,7 @@ constexpr int MERGE_NT = 256, MANY_RECORDS = 8;
 template <typename T, int HD, int NV, int AT, bool ALWAYS_SHARED>
 __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a, int rec_rows, int used) {
     constexpr int LANES = HD / (4 * NV), GROUPS = MERGE_NT / LANES, AHEAD = ALWAYS_SHARED ? 4 : 2;
+    constexpr int SLICES = ALWAYS_SHARED ? GROUPS : MANY_RECORDS, TEAMS = GROUPS / SLICES;  // groups that share a row; rows at a time then
     __shared__ float sm[GROUPS][AT], sl[GROUPS][AT];
     __shared__ float4 so[GROUPS][AT][NV][LANES];
     __shared__ int helps;  // the first CTA of the item that goes on here and has many records
@@ -531,28 +532,28 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
         const PartNote n = notes[first];
         if (n.last == 0) continue;
         const bool shared = ALWAYS_SHARED || n.last - first >= MANY_RECORDS;
-        const int slices = shared ? GROUPS : 1, slice = shared ? group : 0;
-        // rows: AT of all groups at a time, dealt out to the blocks of the item's CTAs, or AT of every group
-        const int at = ALWAYS_SHARED ? (int)blockIdx.y : shared ? ((int)blockIdx.x - first) * (int)gridDim.y + (int)blockIdx.y
-                                                                 : (int)blockIdx.y * GROUPS + group;
-        const int step = (int)gridDim.y * AT * (ALWAYS_SHARED ? 1 : shared ? n.last - first + 1 : GROUPS);
-        for (int r0 = at * AT; r0 < rec_rows; r0 += step) {
+        const int slices = shared ? SLICES : 1, slice = shared ? group % SLICES : 0;
+        // rows: AT of every team at a time, dealt out to the blocks of the item's CTAs, or AT of every group
+        const int teams = shared ? TEAMS : GROUPS, team = shared ? group / SLICES : group;
+        const int turns_of = shared && !ALWAYS_SHARED ? n.last - first + 1 : 1;
+        const int begin = ((turns_of == 1 ? 0 : (int)blockIdx.x - first) * (int)gridDim.y + (int)blockIdx.y) * teams * AT;
+        auto is_row = [&](int row) { return row < rec_rows && (row & 127) < used && n.tile_row + (row >> 7) * used + (row & 127) < n.rows; };
+        for (int b0 = begin; b0 < rec_rows; b0 += turns_of * (int)gridDim.y * teams * AT) {
             Part mine[AT];
             int rows[AT], item_rows[AT];
             bool any = false;
 #pragma unroll
             for (int i = 0; i < AT; ++i) {
-                const int row = r0 + i, item_row = n.tile_row + (row >> 7) * used + (row & 127);
-                const bool real = row < rec_rows && (row & 127) < used && item_row < n.rows;
-                any |= real;
-                rows[i] = real ? row : -1;
-                item_rows[i] = item_row;
+                const int row = b0 + team * AT + i;
+                any |= is_row(row);
+                rows[i] = is_row(row) ? row : -1;
+                item_rows[i] = n.tile_row + (row >> 7) * used + (row & 127);
                 mine[i].m = -INFINITY;
                 mine[i].l = 0.0f;
 #pragma unroll
                 for (int v = 0; v < NV; ++v) mine[i].o[v] = make_float4(0, 0, 0, 0);
             }
-            if (!any) continue;  // the same for all groups that share them
+            if (shared && !ALWAYS_SHARED ? !__syncthreads_or(any) : !any) continue;
             for (int c0 = first + slice; c0 <= n.last; c0 += AHEAD * slices) {
                 int there[AHEAD];
                 Part read[AHEAD][AT];
@@ -581,8 +582,7 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
                         }
                     }
             }
-            if (shared) {  // group g joins and writes the g-th of the rows
-                __syncthreads();
+            if (shared) {  // group i of a team joins and writes the i-th of its rows
 #pragma unroll
                 for (int i = 0; i < AT; ++i) {
 #pragma unroll
@@ -592,16 +592,17 @@ __global__ void __launch_bounds__(MERGE_NT) paged_merge_kernel(const PagedArgs a
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < AT; ++i) {
-                    if (i != group % AT || group >= AT) {
+                    if (i != slice) {
                         rows[i] = -1;
                         continue;
                     }
-                    for (int g = 0; g < GROUPS; ++g) {
+                    for (int g = 0; g < SLICES; ++g) {
                         Part other;
-                        other.m = sm[g][i];
-                        other.l = sl[g][i];
+                        const int at = team * SLICES + g;
+                        other.m = sm[at][i];
+                        other.l = sl[at][i];
 #pragma unroll
-                        for (int v = 0; v < NV; ++v) other.o[v] = so[g][i][v][lane];
+                        for (int v = 0; v < NV; ++v) other.o[v] = so[at][i][v][lane];
                         if (g == 0) mine[i] = other;
                         else join(mine[i], other);
                     }
