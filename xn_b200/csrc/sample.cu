@@ -123,6 +123,7 @@ struct Shared {
     int found_bin;
 };
 
+
 // A token's place in the falling order: its logit's bits, ordered, and the complement of its index.
 __device__ __forceinline__ unsigned order_of(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);  // -0 as 0
@@ -188,10 +189,29 @@ __device__ __noinline__ ulonglong2 block_scan(Shared &s, u64 x) {
     const u64 sum = __shfl_sync(0xffffffffu, w, SM_WARPS - 1), before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
     return make_ulonglong2((warp ? before : 0) + inc - x, sum);
 }
-// Sorts the first `count` values of the list in falling order: value e of thread tid is the EACH * tid + e-th.  Exchanges within a
-// thread, within a warp by shuffles, and beyond through `taken`; only the warps that hold any take part.
+// Sorts the first `count` values of the list, all different, in falling order.
 __device__ __noinline__ void sort_list(Shared &s, int count) {
     const int tid = threadIdx.x;
+    if (count <= SM_NT) {
+        // One or two threads a value: how many are larger is its place.  The time goes with the square of their number; two sorts of 200 to
+        // 250 values take 4 us less than by the steps below.
+        const int parts = count <= SM_NT / 2 ? 2 : 1, i = tid / parts;
+        if (tid == 0) s.list[count] = 0;  // two at a time are looked at
+        __syncthreads();
+        const u64 x = i < count ? s.list[i] : 0;
+        int place = 0;
+#pragma unroll 4
+        for (int j = 2 * (tid % parts); j < count; j += 2 * parts) {
+            place += (s.list[j] > x) + (s.list[j + 1] > x);
+        }
+        if (parts == 2) place += __shfl_xor_sync(0xffffffffu, place, 1);
+        __syncthreads();
+        if (i < count && tid % parts == 0) s.list[place] = x;
+        __syncthreads();
+        return;
+    }
+    // Value e of thread tid is the EACH * tid + e-th.  Exchanges within a thread, within a warp by shuffles, and beyond through `taken`;
+    // only the warps that hold any take part.
     int size = 32 * EACH;
     while (size < count) size <<= 1;
     __syncthreads();
