@@ -321,3 +321,15 @@ def test_broadcast_queries_and_pools(xn, cuda, n):
         wide.check(run(b.q, kk, vv))
     assert torch.equal(xn.attention_paged(b.q, k, v, b.table[:1].expand_as(b.table), b.context, b.scale, query_starts=b.starts, max_query=n),
                        xn.attention_paged(b.q, k, v, b.table[:1].expand_as(b.table).contiguous(), b.context, b.scale, query_starts=b.starts, max_query=n))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("streams,n,heads,kv,ctx", [(1, 5, 8, 2, 90), (3, 40, 8, 2, 200), (2, 37, 3, 1, 600), (4, 100, 6, 2, 131), (6, 24, 24, 24, 24), (1, 300, 8, 1, 300),
+                                                    (49, 17, 1, 1, 50), (50, 17, 1, 1, 50), (2, 600, 2, 2, 1300)])
+def test_small_calls_on_either_side_of_the_line(xn, cuda, streams, n, heads, kv, hd, ctx):
+    """Items of 16 rows from a few to hundreds, over short and long contexts, with tables that fit and tables that have room."""
+    b = Batch(cuda, torch.bfloat16, [(n - i % 2, ctx + 3 * i) for i in range(streams)], heads, kv, hd, 16, spread=0.7)
+    b.check(b.run(xn, max_query=n))
+    b.check(b.run(xn, max_query=n, window=20), window=20)
+    b.table = torch.nn.functional.pad(b.table, (0, 3000), value=-1)
+    b.check(b.run(xn, max_query=n))

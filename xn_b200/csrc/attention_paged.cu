@@ -59,9 +59,16 @@ extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token
     if (max_query > tokens || max_query == 0) max_query = tokens;
     // rows: query heads of one key head times the new tokens.  The streaming kernel reads the keys once for 16 of them and has its first
     // loads on their way sooner; the tensor-memory kernel reads them once for 256.  Measured at head_dim 128 (streaming / tensor
-    // memory, us): 8 rows of 4 key heads, 4 x 30000 keys 30 / 36, 16 x 3000 18 / 25; 16 rows of 2, 4 x 30000 24 / 27, 16 x 3000
-    // 20 / 21, 1 x 1000 13 / 16; 32 rows of 4, 4 x 30000 53 / 37, 16 x 3000 37 / 25, 1 x 1000 13 / 18.
+    // memory, us): 8 rows of 4 key heads, 4 x 30000 keys 30 / 35, 16 x 3000 18 / 25; 16 rows of 2, 4 x 30000 24 / 26, 16 x 3000
+    // 20 / 21, 1 x 1000 13 / 16; 32 rows of 4, 4 x 30000 53 / 36, 16 x 3000 37 / 25, 1 x 1000 13 / 18.
     const size_t rows = max_query * (heads / kv_heads);
-    if (rows > 16 && paged_tc_fits(a)) return launch_paged_tc(dtype, (int)head_dim, a, (cudaStream_t)stream);
+    // More rows take the streaming kernel too where they make few items of 16 rows and few keys are read for them, as far as the tensors'
+    // sizes tell: its way to the first and from the last key is the shorter one.  Items and MB read (streaming / tensor memory, us), at
+    // head_dim 128: 28 and 1.4 13 / 19, 148 and 20 14 / 20, 35 and 27 18 / 19, 192 and 53 25 / 18; at head_dim 64, where fewer of
+    // them outweigh it: 14 and 4.7 15 / 17, 48 and 0.6 12 / 14, 64 and 2.7 14 / 13, 112 and 5.1 18 / 14, 56 and 59 24 / 21.
+    const size_t room = max_pages * page_size, keys = window > 0 && window < room && window + max_query < room ? window + max_query : room;
+    const double items = (double)batch * kv_heads * ((rows + 15) / 16), bytes = items * keys * head_dim * 4;
+    const bool small = items <= (head_dim == 128 ? sm_count() : sm_count() / 3) && bytes <= 32e6;
+    if (rows > 16 && !small && paged_tc_fits(a)) return launch_paged_tc(dtype, (int)head_dim, a, (cudaStream_t)stream);
     return launch_paged_stream(dtype, (int)head_dim, rows > 16 ? 16 : (int)rows, a, (cudaStream_t)stream);
 }

@@ -1,4 +1,4 @@
-// Attention of few query rows over a paged cache: the keys and values stream through once, from HBM.
+// Attention of few query rows over a paged cache, or of small calls: the keys and values stream through once for 16 rows, from HBM.
 //
 // Work is counted in units of 16 keys of one (sequence, tile of rows, key head) item, all items laid end to end, and dealt out
 // evenly to the warps of the machine, whatever the lengths: a long context is shared by many warps, short ones follow one
