@@ -168,3 +168,26 @@ def test_top_p_wherever_its_border_lies(xn, cuda, vocab):
         check(xn, x, u, top_p=p)
         check(xn, x, u, top_p=p, min_p=torch.full((rows,), 0.2, device=cuda), temperature=0.2 + u)
     check(xn, n(1e-37), u, top_p=p, temperature=torch.full((rows,), 1e-38, device=cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [8192, 16411, 70001])
+@pytest.mark.parametrize("rows", [1, 2, 9, 18, 19, 37, 38, 74, 75])
+def test_rows_that_several_ctas_share(xn, cuda, rows, vocab):
+    """Clusters of every size, on a machine that earlier launches still fill, so that the CTAs of a cluster do not begin together: short
+    stretches, rows that end after the first pass beside rows that go on, and rows of nothing."""
+    g = torch.Generator(device=cuda).manual_seed(rows + vocab)
+    x = torch.randn(rows, vocab, generator=g, device=cuda) * 2
+    x[rows // 2] = -torch.inf
+    u = torch.rand(rows, generator=g, device=cuda)
+    kw = settings(rows, cuda, g)
+    check(xn, x, u, **kw)
+    want = xn.sample(x, u, **kw)
+    heads = torch.randn(300, 32, 128, generator=g, device=cuda).bfloat16()
+    pos, freqs = torch.arange(300, device=cuda), xn.rope_frequencies(128, device=cuda)
+    got = []
+    for i in range(20):
+        xn.rope(heads[:1 + 15 * i], pos[:1 + 15 * i], freqs)
+        got.append(xn.sample(x, u, **kw))
+        got.append(xn.sample(x, u, **kw))
+    assert all(torch.equal(t, want) for t in got)

@@ -560,6 +560,8 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
         if (ranks == 1) __syncthreads();
         else cluster.sync();
     };
+    // Completed by the wait ahead of the first store into another CTA's shared memory: by then every CTA of the cluster has started.
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (tid < ROOTS) s.root[tid] = ROOT[tid] * ONE;
     if (tid == 0) s.far = 0;
     dependent_begin();
@@ -597,6 +599,7 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
 #pragma unroll
     for (int o = SM_WARPS / 2; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (ranks > 1) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (tid < ranks) cluster.map_shared_rank(&s, tid)->best[rank] = best;
         cluster.sync();
         for (int q = 0; q < ranks; ++q) best = max(best, s.best[q]);
