@@ -634,10 +634,11 @@ __global__ void __launch_bounds__(SM_NT, 1) sample_kernel(const SampleArgs a, co
         const u64 x = u > 0.0f ? (u64)((double)u * (double)sum) : 0ull;
         return x < sum ? x : sum - 1;
     };
-    // a logit below those of the steps up to this one, and one above those from this one on, whatever was rounded
-    const float width = t / STEPS, slack = 0.01f * width + 1e-6f * fabsf(r.top);
-    auto edge = [&](int step) { return step < 2 * BINS ? r.top - (step + 1) * width * 1.00001f - slack : -INFINITY; };
-    auto upper_edge = [&](int step) { return step ? fminf(r.top - step * width * 0.99999f + slack, r.top) : r.top; };
+    // A logit below those of the steps up to this one, and one not below those from this one on.  A step is off by some 2^-22 of itself; the
+    // rest is exact enough in 64 bits, down to the smallest t, and rounded outwards.
+    const double width = (double)t / STEPS;
+    auto edge = [&](int step) { return step < 2 * BINS ? __double2float_rd((double)r.top - (step + 1) * width * 1.00001) : -INFINITY; };
+    auto upper_edge = [&](int step) { return step ? fminf(__double2float_ru((double)r.top - step * width * 0.99999), r.top) : r.top; };
     auto sums_command = [&](u64 cut) {
         Command c{};
         c.op = OP_SUMS; c.cut = cut;
