@@ -398,12 +398,12 @@ int xn_mm_paged_append(xn_dtype dtype, void *k_pages, void *v_pages, size_t page
                        const int64_t *positions, const double *freqs_or_null, size_t rotated, int interleaved, void *stream);
 /* Attention of the newest tokens of `batch` sequences over the paged cache that already holds their keys and values.
  * Sequence b has the query rows [query_starts[b], query_starts[b + 1]) of q (query_starts null: row b alone) and context[b] keys
- * with them; its row i of n sees key j iff j <= i + context[b] - n and, where window > 0, j > i + context[b] - n - window:
+ * with them; its row i of n sees key j iff j <= i + context[b] - n and, where window > 0 (any size), j > i + context[b] - n - window:
  *   out[t][h] = softmax_j(scale * q[t][h] . k[j][h / (heads / kv_heads)]) v[j][...]
- * A row that sees nothing is zeros; rows of q that belong to no sequence leave out as it is.  16-bit elements, head_dim 64 or
- * 128, any page size, 16-byte aligned tensors with strides in multiples of 8 elements.  Scores, softmax statistics and the output's sum
- * are f32; the probabilities are rounded to the element type for the second product.  max_query: an upper bound of the rows of a
- * sequence, by which the kernel is chosen (0: unknown); results hold for any.
+ * scale is finite and not negative.  A row that sees nothing is zeros; rows of q that belong to no sequence leave out as it is.
+ * 16-bit elements, head_dim 64 or 128, any page size, 16-byte aligned tensors with strides in multiples of 8 elements.  Scores,
+ * softmax statistics and the output's sum are f32; the probabilities are rounded to the element type for the second product.
+ * max_query: an upper bound of the rows of a sequence, by which the kernel is chosen (0: unknown); results hold for any.
  * Lengths and indexes are device memory that the host does not see: a length is bounded by the tensors, and a page index outside
  * [0, num_pages) reads as a page of zeros.  What pages hold beyond a sequence's context is never used.  A key or value inside
  * the context that is not finite makes the rows that see it so (maybe in all of the head's elements), and no others.

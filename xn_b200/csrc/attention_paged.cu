@@ -52,7 +52,7 @@ extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token
     a.page_shift = -1;
     if ((page_size & (page_size - 1)) == 0)
         for (a.page_shift = 0; (size_t)1 << a.page_shift < page_size; ++a.page_shift) {}
-    a.window = (int)(window < 0x3fffffffull ? window : 0x3fffffffull);
+    a.window = window < max_pages * page_size ? (int)window : 0;  // one as wide as the table hides nothing
     a.c = fmaxf(scale * 1.4426950408889634f, 1e-37f);  // above zero: a masked score, -inf, stays -inf
     a.ws = workspace;
     if (!query_starts_or_null) max_query = 1;

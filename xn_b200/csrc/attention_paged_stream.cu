@@ -63,7 +63,7 @@ struct SequenceUnits {
 template <int TR> __device__ __forceinline__ SequenceUnits sequence_units(const PagedArgs &a, int b) {
     SequenceUnits u;
     u.s = load_sequence(a, b);
-    u.lo = a.window ? max(0, u.s.off + 1 - a.window) : 0;
+    u.lo = first_key(a, u.s.off);
     u.base = u.lo / UNIT * UNIT;
     u.U = max(1, (u.s.ctx - u.base + UNIT - 1) / UNIT);  // rows that see nothing get their zeros from an empty unit
     u.tiles = (int)(((long long)u.s.n * a.group + TR - 1) / TR);
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                 item_begin = cc.pos - (unsigned)cc.unit;
                 const int rows = (int)min((long long)cc.u.s.n * a.group - (long long)cc.tile * TR, (long long)TR);
                 sure_hi = cc.u.s.off + (int)((unsigned)(cc.tile * TR) / (unsigned)a.group);
-                sure_lo = a.window ? cc.u.s.off + (int)((unsigned)(cc.tile * TR + rows - 1) / (unsigned)a.group) - a.window + 1 : 0;
+                sure_lo = first_key(a, cc.u.s.off + (int)((unsigned)(cc.tile * TR + rows - 1) / (unsigned)a.group));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const int rq = nt * 8 + (lane >> 2);  // the row of this lane's Q fragments
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_stream_kernel(const Paged
                         const int rs = nt * 8 + (lane & 3) * 2 + e;  // the row of this lane's scores
                         const int i = (int)((unsigned)(cc.tile * TR + rs) / (unsigned)a.group);
                         hi_key[nt][e] = rs < rows ? min(cc.u.s.ctx - 1, cc.u.s.off + i) : -1;
-                        lo_key[nt][e] = a.window ? cc.u.s.off + i - a.window + 1 : 0;
+                        lo_key[nt][e] = first_key(a, cc.u.s.off + i);
                         m[nt][e] = -INFINITY;
                         l[nt][e] = 0.0f;
                     }

@@ -64,7 +64,7 @@ __device__ __forceinline__ TcItem tc_item(const TcArgs &a, int n, int off, int i
     i.ntok = min(n - i.tok0, 2 * a.tile_tokens);
     i.dual = i.ntok > a.tile_tokens;
     const int last = off + i.tok0 + i.ntok - 1;
-    i.lo = a.p.window ? max(0, off + i.tok0 - a.p.window + 1) : 0;
+    i.lo = first_key(a.p, off + i.tok0);
     i.kb0 = i.lo / KEYS;
     i.kb1 = max(last >= 0 ? last / KEYS + 1 : 0, i.kb0 + 1);
     return i;
@@ -101,7 +101,7 @@ struct Sure {
     int lo, hi, last;
     __device__ __forceinline__ Sure(const TcArgs &a, const Segment &g) {
         const int end = min(g.tok0 + (1 + g.dual) * a.tile_tokens, g.n);
-        lo = a.p.window ? g.off + end - a.p.window : 0;
+        lo = first_key(a.p, g.off + end - 1);
         hi = min(g.ctx - 1, g.off + g.tok0);
         last = min(g.ctx, g.off + end) - 1;
     }
@@ -596,7 +596,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const bool real = r < tile_rows && tok < g.n && !dry;
             const bool any_real = __any_sync(0xffffffffu, real) || dry;
             const int horizon = min(ctx - 1, g.off + tok);
-            const int low = p.window ? g.off + tok - p.window + 1 : 0;
+            const int low = first_key(p, g.off + tok);
             float m = real ? -INFINITY : 0.0f;  // rows of nobody never move their reference
             u64 l2[2] = {0, 0};
             bool begun = false;

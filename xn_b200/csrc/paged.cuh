@@ -21,7 +21,7 @@ struct PagedArgs {
     long long table_stride;
     int tokens, batch, heads, kv_heads, group;
     int num_pages, page_size, page_shift, max_pages;  // page_shift: log2(page_size), or -1
-    int window;
+    int window;  // 0, or fewer keys than a table holds
     float c;  // scale * log2(e)
     void *ws;
     int parts;  // CTAs that share the work
@@ -45,6 +45,9 @@ __device__ __forceinline__ Sequence load_sequence(const PagedArgs &a, int b) {
     s.off = s.ctx - s.n;
     return s;
 }
+
+// The first key that a row sees whose last is `last`.  Windows go up to 2^31: last - window + 1 alone could leave 32 bits.
+__device__ __forceinline__ int first_key(const PagedArgs &a, int last) { return a.window && last >= a.window ? last - a.window + 1 : 0; }
 
 // A row's result over a part of its keys: the sum of p v (head_dim floats), the maximum m of its scaled scores and the sum l of
 // p = 2^(score - m).  CTA c of `parts` writes the part of the item that began before it into record 0 and the part of the one that it
