@@ -470,6 +470,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
         } else if (warp == 1) {
             // ---- MMA issuer ----
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // ahead of the first wait: its limit is not for what earlier kernels take
             if (elect_one()) {
                 bool ok = true;
                 unsigned nk = 0, nv = 0, np[2] = {0, 0};
