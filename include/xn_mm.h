@@ -380,7 +380,8 @@ int xn_mm_kv_append2(xn_dtype dtype, void *k_cache, void *v_cache, const void *k
  * page * page_size + row.
  * ------------------------------------------------------------------------------------------ */
 /* Rotary positions: dst[t][h] = src[t][h] with pair j of the first `rotated` elements turned by positions[t] * freqs[j] radians
- * (rotated / 2 frequencies, 64-bit: the angle is formed in 64 bits, so far positions lose nothing).  interleaved: pairs are
+ * (rotated / 2 frequencies, 64-bit).  The angle is off by 2^-23 radians whatever the position, up to positions of 2^53 and angles
+ * of 2^52 half turns: its product is kept in twice 64 bits until whole turns are off.  interleaved: pairs are
  * elements (2 j, 2 j + 1) (rope_i, xn-core/src/backend.rs), otherwise (j, j + rotated / 2) (rope).  The rest of each head of head_dim
  * elements is copied.  f32 math, one rounding.  Any strides with contiguous heads; dst may be src with the same strides,
  * and must not overlap it otherwise. */

@@ -5,10 +5,12 @@
 // with x0, x1 side by side (elements 2 j, 2 j + 1) or half the rotated part apart (j, j + pairs); what lies behind the rotated
 // part of the head is copied.  Products and sums in f32, one rounding to the element type.
 //
-// The angle is formed in 64 bits, as turns: t = position * (freqs[j] / 2 pi), less its nearest integer, and only the rest, at
-// most half a turn, is rounded to f32 for the sine and cosine.  A product in f32 would be off by position * 2^-24 radians:
-// 0.06 at position 10^6, where this is off by 2^-24 whatever the position.  It needs no table of a length that somebody has to
-// know beforehand, and one thread's pairs keep their sine and cosine for all the heads that the thread turns.
+// The angle is formed as half turns, t = position * (freqs[j] / pi), less the nearest even number, and only the rest, at most one
+// half turn, is rounded to f32 for the sine and cosine.  A product in f32 would be off by position * 2^-24 radians: 0.06 at
+// position 10^6; one in 64 bits by position * 2^-53.  Here freqs[j] / pi and t are held in two numbers of 64 bits each, the second what
+// the first one's rounding left (products with fma), so that the rest is off by 2^-25 half turns whatever the position, as long as t
+// is below 2^52 and the position a whole number that 64-bit floats hold (2^53).  It needs no table of a length that somebody
+// has to know beforehand, and one thread's pairs keep their sine and cosine for all the heads that the thread turns.
 //
 // Bound: memory.  A thread moves a chunk of 2 x 16 bytes per head (16-bit elements: 8 pairs, f32: 4) where the sizes and the
 // alignment allow it, single pairs otherwise; several heads share its sines and cosines.  Measured: 4001 tokens x 16 heads of 64 in
@@ -80,9 +82,11 @@ __global__ void __launch_bounds__(ROPE_NT) rope_kernel(const RopeArgs a) {
         const double pos = (double)a.positions[token];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            // half turns, less the nearest even number of them: a sum with 1.5 * 2^53 is rounded to one
-            const double t = pos * (a.freqs[chunk * V + j] * 0.3183098861837907), k = t + 13510798882111488.0;
-            sincospif((float)(t - (k - 13510798882111488.0)), &sn[j], &cs[j]);
+            constexpr double INV_PI = 0.3183098861837907, REST = -1.9678676675182486e-17;  // 1 / pi in two numbers
+            const double f = a.freqs[chunk * V + j], c = f * INV_PI, c_rest = fma(f, REST, fma(f, INV_PI, -c));
+            const double t = pos * c, t_rest = fma(pos, c_rest, fma(pos, c, -t));
+            const double k = t + 13510798882111488.0;  // a sum with 1.5 * 2^53 is rounded to an even number
+            sincospif((float)(t - (k - 13510798882111488.0) + t_rest), &sn[j], &cs[j]);
         }
     }
     // the two runs of the chunk within its head, with and without rotation

@@ -321,7 +321,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interlea
          out: torch.Tensor | None = None) -> torch.Tensor:
     """x [tokens, heads, head_dim] (any strides) with the first ``2 len(freqs)`` elements of each head turned by their token's
     position (int64 [tokens]): pairs side by side (``interleaved``: the reference's rope_i) or half the rotated part apart (rope).
-    freqs: f64, see rope_frequencies.  The angle is formed in 64 bits.  ``out`` may be x itself."""
+    freqs: f64, see rope_frequencies.  Far positions lose nothing (xn_mm_rope).  ``out`` may be x itself."""
     return _host.rope(x, positions, freqs, interleaved, out)
 
 
