@@ -1,4 +1,5 @@
 // Entry points of attention over a paged cache: checks, and which kernel a call gets.
+#include <float.h>
 #include <math.h>
 
 #include "paged.cuh"
@@ -53,7 +54,7 @@ extern "C" int xn_mm_attention_paged(xn_dtype dtype, void *out, size_t out_token
     if ((page_size & (page_size - 1)) == 0)
         for (a.page_shift = 0; (size_t)1 << a.page_shift < page_size; ++a.page_shift) {}
     a.window = window < max_pages * page_size ? (int)window : 0;  // one as wide as the table hides nothing
-    a.c = fmaxf(scale * 1.4426950408889634f, 1e-37f);  // above zero: a masked score, -inf, stays -inf
+    a.c = fminf(fmaxf(scale * 1.4426950408889634f, 1e-37f), FLT_MAX);  // above zero, so that a masked score, -inf, stays -inf, and finite
     a.ws = workspace;
     if (!query_starts_or_null) max_query = 1;
     if (max_query > tokens || max_query == 0) max_query = tokens;
