@@ -407,7 +407,8 @@ int xn_mm_paged_append(xn_dtype dtype, void *k_pages, void *v_pages, size_t page
  * max_query: an upper bound of the rows of a sequence, by which the kernel is chosen (0: unknown); results hold for any.
  * Lengths and indexes are device memory that the host does not see: a length is bounded by the tensors, and a page index outside
  * [0, num_pages) reads as a page of zeros.  What pages hold beyond a sequence's context is never used.  A key or value inside
- * the context that is not finite makes the rows that see it so (maybe in all of the head's elements), and no others.
+ * the context that is not finite makes the rows that see it so (maybe in all of the head's elements), and no others; where a row's
+ * score is -inf, that key weighs nothing in the row, and a row of such scores only is zeros.
  * out overlaps none of the other tensors.  workspace: xn_mm_attention_paged_workspace_bytes(head_dim) bytes (a number of the current
  * device's) of device memory, 256-byte aligned, owned by the caller; calls that may overlap need one each. */
 size_t xn_mm_attention_paged_workspace_bytes(size_t head_dim);

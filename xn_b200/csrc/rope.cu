@@ -12,15 +12,16 @@
 // is below 2^52 and the position a whole number that 64-bit floats hold (2^53).  It needs no table of a length that somebody
 // has to know beforehand, and one thread's pairs keep their sine and cosine for all the heads that the thread turns.
 //
-// Bound: memory.  A thread moves a chunk of 2 x 16 bytes per head (16-bit elements: 8 pairs, f32: 4) where the sizes and the
+// Bound: latency.  A thread reads its position and its frequencies and takes sines before it asks for its heads (caches cold, DRAM is busy
+// for a fifth of the time and the issue slots for less than a half).  It moves a chunk of 2 x 16 bytes per head (16-bit elements: 8 pairs, f32: 4) where the sizes and the
 // alignment allow it, single pairs otherwise; several heads share its sines and cosines.  Measured: 4001 tokens x 16 heads of 64 in
-// f32, 16 elements turned, 7.6 us (4.3 TB/s); append of 4096 tokens x (16 + 16 + 16) heads of 64 in f16 11.2 us (4.5 TB/s).
+// f32, 16 elements turned, 7.8 us (4.2 TB/s); append of 4096 tokens x (16 + 16 + 16) heads of 64 in f16 11.9 us (4.2 TB/s).
 #include "common.cuh"
 
 namespace xn {
 namespace {
 
-constexpr int ROPE_NT = 128;  // 256: 13.2 us instead of 11.2 for the f16 append above, whose last blocks run alone for longer
+constexpr int ROPE_NT = 128;  // 256: 13.2 us instead of 11.2 for the f16 append above (before its angles were kept whole), whose last blocks run alone for longer
 
 // One tensor [tokens, heads, head_dim] of the call: where it is read and where it goes.  dst == null marks an unused one.
 struct RopePart {

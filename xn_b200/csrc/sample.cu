@@ -27,8 +27,8 @@
 //   are too many), which give the exact end;
 //   the kept weights of every warp's stretch of the row, and the stretch that the draw falls into.
 // Bound: the latency of the passes for few rows; for many, the instructions of the weights, the histogram's additions in shared
-// memory and the reads.  Measured, all in us: one row of 32000 f32, all filters, 20; 24 rows of 50000 bf16 35; 64 rows of 128001
-// f32, top-p, 72 (105 with the exact weights put into the histogram, which took two passes over them); no filter 48.
+// memory and the reads.  Measured, all in us: one row of 32000 f32, all filters, 21 to 26; 24 rows of 50000 bf16 35; 64 rows of 128001
+// f32, top-p, 75 (105 with the exact weights put into the histogram, which took two passes over them); no filter 48.
 #include <cooperative_groups.h>
 
 #include <type_traits>

@@ -321,7 +321,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interlea
          out: torch.Tensor | None = None) -> torch.Tensor:
     """x [tokens, heads, head_dim] (any strides) with the first ``2 len(freqs)`` elements of each head turned by their token's
     position (int64 [tokens]): pairs side by side (``interleaved``: the reference's rope_i) or half the rotated part apart (rope).
-    freqs: f64, see rope_frequencies.  Far positions lose nothing (xn_mm_rope).  ``out`` may be x itself."""
+    freqs: f64, see rope_frequencies.  Far positions lose nothing (xn_mm_rope).  ``out`` may be x itself, and overlaps it not
+    otherwise."""
     return _host.rope(x, positions, freqs, interleaved, out)
 
 
@@ -344,13 +345,13 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Query heads share the pools' kv_heads evenly.  Row i of n sees key j iff j <= i + context - n, with a window > 0 only the last
     `window` of those; a row that sees nothing is zeros.  Rows behind the last sequence are not written.  max_query: the longest
     sequence's rows where the program knows it (the tensors are on the device); it decides which kernel runs, not what it
-    gives.  f16 / bf16, head_dim 64 or 128, any page size."""
+    gives.  f16 / bf16, head_dim 64 or 128, any page size; scale finite and not negative; out overlaps no other tensor of the call."""
     return _host.attention_paged(q, k_pages, v_pages, page_table, context, scale, query_starts, max_query, window, out)
 
 
 def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
            top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None) -> torch.Tensor:
-    """The next token (int64) of every row of logits [rows, vocabulary], from uniform [rows] in [0, 1) (xn_mm_sample): the rows'
+    """The next token (int64) of every row of logits [rows, vocabulary up to 2^20], from uniform [rows] in [0, 1) (xn_mm_sample): the rows'
     temperature (f32 [rows]; not positive: the largest logit), top_k (int32; 0: off), top_p (f32; 1: off) and min_p (f32; 0: off), in this order.
     The draw walks the kept tokens in order of index; sums are exact, so equal inputs give equal tokens."""
     return _host.sample(logits, uniform, temperature, top_k, top_p, min_p)
